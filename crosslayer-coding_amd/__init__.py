@@ -8,7 +8,7 @@ import it as ``crosslayer_coding_amd`` (the alias module next to this directory)
 """
 
 from . import _native, engine  # noqa: F401
-from . import activations, base, build, config, decoder, encoder, evaluator, feed, optim, parallel, registry, synth, theta  # noqa: F401
+from . import activations, base, build, config, decoder, encoder, evaluator, feed, mx, optim, parallel, registry, synth, theta  # noqa: F401
 from .activations import BatchTopK, JumpReLU, TokenTopK
 from .clt import CrossLayerTranscoder
 from .config import CLTConfig
@@ -16,9 +16,11 @@ from .engine import SurvivorList
 from .optim import CLTAdam
 from .evaluator import CLTEvaluator, DeadFeatureTracker
 from .feed import DeviceActivationFeed
+from .mx import MXActivationCache, MXTensor
 from .registry import ACTIVATION_REGISTRY, get_activation_fn, register_activation_fn
 
 __all__ = [
     "CrossLayerTranscoder", "CLTConfig", "CLTAdam", "CLTEvaluator", "DeadFeatureTracker", "DeviceActivationFeed", "BatchTopK", "TokenTopK", "JumpReLU", "SurvivorList",
+    "MXTensor", "MXActivationCache",
     "ACTIVATION_REGISTRY", "get_activation_fn", "register_activation_fn",
 ]

@@ -129,6 +129,13 @@ _SIGNATURES = {
     "clt_probe_gather": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _int, _vp, _vp]),
     "clt_feed_gather": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _int, _vp, _vp, _vp, _vp, _f64, _vp, _vp,
                               _i64, _i64, _int, _vp]),
+    "clt_mx_row_bytes": (_i64, [_i64, _int]),
+    "clt_mx_quantise": (_int, [_vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp]),
+    "clt_mx_dequantise": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _i64, _int, _vp]),
+    "clt_mx_cache_write": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _int, _i64, _i64, _i64, _i64, _int, _vp, _vp, _i64, _vp, _vp]),
+    "clt_mx_cache_read": (_int, [_vp, _vp, _i64, _int, _vp, _int, _i64, _i64, _i64, _i64, _int, _vp, _vp, _vp, _vp, _f64, _vp, _vp,
+                                 _i64, _i64, _int, _vp]),
+    "clt_mx_encode": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _vp]),
     "clt_survivor_metrics": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, ctypes.c_float, _vp, _vp, _vp]),
     "clt_dead_feature_update": (_int, [_vp, _vp, _i64, _vp]),
     "clt_reconstruction_stats_workspace_bytes": (_sz, [_i64, _i64]),

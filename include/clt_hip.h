@@ -878,6 +878,60 @@ int clt_feed_gather(const void *src, int src_dtype, int64_t src_rows, int64_t sr
                     const float *mean_tg, const float *std_tg, double scale, void *x_out,
                     void *tgt_out, int64_t out_row0, int64_t T, int out_dtype, void *stream);
 
+/* ---- microscaled formats ---------------------------------------------------------
+ * No counterpart in the reference: 8- and 4-bit forms of what it keeps in 16 or 32 bits.
+ * 32 neighbouring elements of a row form a block and share a scale 2^(s - 127), s one byte:
+ *   s = biased exponent of the block's largest magnitude - largest exponent of the element type,
+ *   held in 0 .. 254; 255 where the block holds an infinity or a NaN: all of it reads back as NaN.
+ * The elements are stored as v 2^(127 - s), rounded to nearest even, beyond the largest value to it.
+ *   CLT_MXFP4    16 bytes per block   0 0.5 1 1.5 2 3 4 6 and their negatives, the even element in the low half of a byte
+ *   CLT_MXFP8    32 bytes per block   e4m3, up to 448
+ *   CLT_MXINT8   32 bytes per block   two's complement in 64ths, -127/64 .. 127/64
+ * A row of d elements has ceil(d / 32) blocks (the last one filled up with zeros): clt_mx_row_bytes(d, fmt) bytes of codes
+ * (0: not a format) and ceil(d / 32) bytes of scales; rows follow one another without gaps, codes begin 16-byte aligned
+ * (else CLT_ERR_ALIGN).  d up to 262144, at most 2^31 - 1 rows a call.
+ *
+ * clt_mx_quantise / clt_mx_dequantise: n rows of d elements (dtype CLT_F32 / CLT_BF16 / CLT_F16), row_stride elements
+ *   apart, to codes and scales and back (fp32, one rounding to dtype).
+ *
+ * clt_mx_cache_write / clt_mx_cache_read: a store of activations, codes [L][2][rows][row bytes] and scales
+ *   [L][2][rows][blocks] (inputs and targets of every layer; clt/training/data/manifest_activation_store.py:555-560 keeps
+ *   the same tensors in 16 or 32 bits).
+ *   write: row j of x and tgt (n rows of d elements, row_stride apart, layers layer_stride apart) is quantised into row
+ *     row_index[j] of the store (index_bits 32 or 64, device), or first + j when row_index is NULL.  Where several name
+ *     one row it keeps the last; `owner` (int32 [rows], contents arbitrary, needed with row_index) is scratch of the call.
+ *     A row number outside [0, rows) is not written.  All other rows stay as they are.
+ *   read: rows [out_row0, out_row0 + n) of x_out, tgt_out [L][T][d] (out_dtype) from rows row_index[j] or first + j;
+ *     normalisation and arguments as in clt_feed_gather.  A row number outside [0, rows) is not read: its row is NaN.
+ *
+ * clt_mx_encode: pre[l] = x[l] . w[l]^T + b[l] with both operands in CLT_MXFP4 (x [L][T], w [L][F] rows of d elements):
+ *   exact products, fp32 sums, the bias added in fp32, one rounding to dtype (that of bias and pre; bias may be NULL).
+ *   pre rows are pre_row_stride >= F elements apart.  What clt_encode computes from 16- or 32-bit operands
+ *   (clt/models/parallel.py:286).  T up to 2^20, F up to 2^30, L up to 65535.
+ */
+#define CLT_MXFP4 0
+#define CLT_MXFP8 1
+#define CLT_MXINT8 2
+
+int64_t clt_mx_row_bytes(int64_t d, int fmt);
+int clt_mx_quantise(const void *src, int64_t n, int64_t d, int64_t row_stride, int dtype, int fmt,
+                    void *codes, uint8_t *scales, void *stream);
+int clt_mx_dequantise(const void *codes, const uint8_t *scales, int64_t n, int64_t d, int fmt,
+                      void *dst, int64_t row_stride, int dtype, void *stream);
+int clt_mx_cache_write(const void *x, const void *tgt, int64_t layer_stride, int64_t row_stride,
+                       int dtype, const void *row_index, int index_bits, int64_t first, int64_t n,
+                       int64_t d, int64_t L, int fmt, void *codes, uint8_t *scales, int64_t rows,
+                       int32_t *owner, void *stream);
+int clt_mx_cache_read(const void *codes, const uint8_t *scales, int64_t rows, int fmt,
+                      const void *row_index, int index_bits, int64_t first, int64_t n, int64_t d,
+                      int64_t L, int norm_mode, const float *mean_in, const float *std_in,
+                      const float *mean_tg, const float *std_tg, double scale, void *x_out,
+                      void *tgt_out, int64_t out_row0, int64_t T, int out_dtype, void *stream);
+int clt_mx_encode(const void *x_codes, const uint8_t *x_scales, const void *w_codes,
+                  const uint8_t *w_scales, const void *bias, void *pre, int64_t T, int64_t d,
+                  int64_t F, int64_t L, int64_t b_layer_stride, int64_t pre_layer_stride,
+                  int64_t pre_row_stride, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
