@@ -135,7 +135,8 @@ _SIGNATURES = {
     "clt_mx_cache_write": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _int, _i64, _i64, _i64, _i64, _int, _vp, _vp, _i64, _vp, _vp]),
     "clt_mx_cache_read": (_int, [_vp, _vp, _i64, _int, _vp, _int, _i64, _i64, _i64, _i64, _int, _vp, _vp, _vp, _vp, _f64, _vp, _vp,
                                  _i64, _i64, _int, _vp]),
-    "clt_mx_encode": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _vp]),
+    "clt_mx_encode_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _int]),
+    "clt_mx_encode": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _vp, _sz, _vp]),
     "clt_survivor_metrics": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, ctypes.c_float, _vp, _vp, _vp]),
     "clt_dead_feature_update": (_int, [_vp, _vp, _i64, _vp]),
     "clt_reconstruction_stats_workspace_bytes": (_sz, [_i64, _i64]),

@@ -96,7 +96,8 @@ __device__ __forceinline__ MxPiece mx_piece(uint32_t pieces, uint32_t magic) {
   return {(int64_t)(row0 + dj), at - dj * pieces};
 }
 
-// grid: x = groups of pieces, y = layer * kinds + kind.  Four lanes hold a block and agree on its scale.
+// grid: x = groups of pieces, y = layer * kinds + kind.  Four lanes hold a block and agree on its scale.  `blocks` of a stored row: those
+// behind d are zeros.
 template <typename T, int FMT, bool VEC>
 __global__ __launch_bounds__(MX_THREADS) void k_mx_write(const T *__restrict__ src0, const T *__restrict__ src1, int64_t layer_stride,
                                                          int64_t row_stride, int kinds, int64_t n, int64_t d, uint32_t blocks,
@@ -293,13 +294,272 @@ __global__ __launch_bounds__(256) void k_mx_project(const uint8_t *__restrict__ 
   }
 }
 
+// ---- the projection of a batch ------------------------------------------------------------------------------------
+// Tiles of BM tokens x 256 features, one persistent workgroup of 8 wavefronts (4 along the tokens, 2 along the features) per CU.
+// A stage is 128 elements of K: 64 bytes of codes and 4 of scales per row, brought straight into one of four buffers in
+// LDS, chunk c of row r at chunk position c ^ ((r >> 2) & 3), so that the 16 rows of a fragment read lie in all banks.  The
+// stages of all of a workgroup's tiles form one sequence: at the barrier in front of a stage the next one has landed too,
+// and the third after it is asked for, so a load has two stages to arrive, the fragments of the next stage are read under
+// the products of this one, and the first stages of the next tile travel during the last ones of this tile.
+constexpr int TN = 256;                       // features of a tile
+constexpr int TW = 8;                         // wavefronts
+constexpr int TROW = 64;                      // bytes of codes per row and stage
+constexpr int TBUF = 4;
+constexpr int PARK = 2048;                    // bytes of a wavefront's piece of the output tile on its way out
+
+// vmcnt(n), everything else unconstrained
+constexpr int wait_vm(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0F70; }
+
+__device__ __forceinline__ uint32_t mx_lds(const void *p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
+}
+// 16 or 4 bytes per lane from base + off straight into LDS, lane i at at + 16 i or 4 i.  Not counted by the compiler: the
+// waits are written out.
+__device__ __forceinline__ void mx_fill16(const void *base, uint32_t off, uint32_t at) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(at) : "memory");
+}
+__device__ __forceinline__ void mx_fill4(const void *base, uint32_t off, uint32_t at) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "{m0}"(at) : "memory");
+}
+
+struct TileArgs {
+  const uint8_t *xc, *xs, *wc, *ws;           // x rows hold whole stages (zeros behind the end), so do all scale rows
+  int M, N, tiles_m, tiles_n, total, per_xcd;
+  int stages, xpitch, wpitch, spitch, wblocks;   // bytes of a row of codes, of scales; blocks of W that are there
+  int64_t bs, ps, pre_row;
+};
+
+template <typename OutT, int MG>
+__global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_mx_project_tiles(
+    TileArgs a, const OutT *__restrict__ bias, OutT *__restrict__ pre) {
+  constexpr int BM = 64 * MG;                              // tokens of a tile; a wavefront takes 16 MG x 128
+  constexpr int XI = BM / 16, XPW = XI >= TW ? XI / TW : 1;   // loads of 16 rows of x; per wavefront (some twice where there are few)
+  constexpr int SI = (BM + TN) / 64;                       // loads of the scales of 64 rows
+  constexpr int LOADS = XPW + 2 + 1;                       // of a stage, per wavefront
+  constexpr int STAGE = (BM + TN) * TROW, SST = (BM + TN) * 4;
+  constexpr int HF = 128 / (int)sizeof(OutT);              // features of a parked piece: rows of 128 bytes
+  constexpr int STORES = MG * (128 / HF) * 2;              // stores of a whole tile, per wavefront
+  static_assert(LOADS + STORES < 64, "the wait counter holds 63");
+  __shared__ __attribute__((aligned(16))) unsigned char ring[TBUF * STAGE];
+  __shared__ __attribute__((aligned(16))) unsigned char sring[TBUF * SST];
+  __shared__ __attribute__((aligned(16))) unsigned char parked[TW * PARK];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave & 3, wn = wave >> 2, l15 = lane & 15, lq = lane >> 4;
+  const uint32_t ring0 = mx_lds(ring), sring0 = mx_lds(sring);
+
+  // Block b runs on XCD b % 8 and takes every (gridDim / 8)-th of that XCD's share of the tiles, a run of them in an order
+  // that goes through 8 feature tiles for each token tile: the W tiles stay in the XCD's L2 while the tokens pass.
+  struct At { int layer, m0, n0; };
+  auto locate = [&](int t) {
+    const int per = a.tiles_m * a.tiles_n;
+    At at;
+    at.layer = t / per;
+    t -= at.layer * per;
+    const int g = t / (8 * a.tiles_m), r = t - g * 8 * a.tiles_m;
+    const int cnt = min(8, a.tiles_n - g * 8);
+    const int tm = r / cnt;
+    at.m0 = tm * BM;
+    at.n0 = (g * 8 + r - tm * cnt) * TN;
+    return at;
+  };
+  const int step = (int)gridDim.x >> 3;
+  const int last_tile = min((((int)blockIdx.x & 7) + 1) * a.per_xcd, a.total);
+  int tile = ((int)blockIdx.x & 7) * a.per_xcd + ((int)blockIdx.x >> 3);
+  if (tile >= last_tile) return;
+
+  // ---- the loader: where its next stage comes from
+  int in_tile = tile, in_stage = 0;
+  uint32_t in_buf = 0, xo[XPW], wo[2], so;
+  const uint8_t *in_x, *in_w, *in_s;
+  const uint32_t chunk = (uint32_t)((lane & 3) ^ ((lane >> 4) & 3));
+  const int sunit = wave % SI;
+  auto aim = [&]() {
+    const At at = locate(in_tile);
+    in_x = a.xc + ((int64_t)at.layer * a.M + at.m0) * a.xpitch;
+    in_w = a.wc + ((int64_t)at.layer * a.N + at.n0) * a.wpitch;
+    const int xl = a.M - 1 - at.m0, wl = a.N - 1 - at.n0;     // rows past the end repeat the last one
+#pragma unroll
+    for (int i = 0; i < XPW; ++i) xo[i] = (uint32_t)min(((wave * XPW + i) % XI) * 16 + (lane >> 2), xl) * (uint32_t)a.xpitch + chunk * 16u;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) wo[i] = (uint32_t)min((wave * 2 + i) * 16 + (lane >> 2), wl) * (uint32_t)a.wpitch;
+    const bool of_x = sunit * 64 < BM;
+    in_s = of_x ? a.xs + ((int64_t)at.layer * a.M + at.m0) * a.spitch : a.ws + ((int64_t)at.layer * a.N + at.n0) * a.spitch;
+    so = (uint32_t)min((of_x ? sunit * 64 : sunit * 64 - BM) + lane, of_x ? xl : wl) * (uint32_t)a.spitch;
+  };
+  auto load_stage = [&]() {
+    const uint32_t at = ring0 + in_buf * STAGE, sat = sring0 + in_buf * SST;
+#pragma unroll
+    for (int i = 0; i < XPW; ++i) mx_fill16(in_x + (int64_t)in_stage * TROW, xo[i], at + (uint32_t)((wave * XPW + i) % XI) * 1024u);
+    const uint32_t k16 = (uint32_t)min(in_stage * 4 + (int)chunk, a.wblocks - 1) * 16u;   // x is zero where W repeats its last block
+#pragma unroll
+    for (int i = 0; i < 2; ++i) mx_fill16(in_w, wo[i] + k16, at + BM * TROW + (uint32_t)(wave * 2 + i) * 1024u);
+    mx_fill4(in_s + (int64_t)in_stage * 4, so, sat + (uint32_t)sunit * 256u);
+    in_buf = (in_buf + 1) & (TBUF - 1);
+    if (++in_stage == a.stages) {
+      in_stage = 0;
+      if (in_tile + step < last_tile) in_tile += step;         // behind the last tile: once more, for nobody
+      aim();
+    }
+  };
+
+  // ---- fragments: row l15 of each group of 16, its block lq
+  const uint32_t pos = (uint32_t)(lq ^ (l15 >> 2)) * 16u;
+  const uint32_t xat = (uint32_t)(wm * 16 * MG + l15) * TROW + pos, wat = (uint32_t)(BM + wn * 128 + l15) * TROW + pos;
+  const uint32_t xsat = (uint32_t)(wm * 16 * MG + l15) * 4 + lq, wsat = (uint32_t)(BM + wn * 128 + l15) * 4 + lq;
+  uint4 fx[MG], fw[2][2];
+  uint32_t sx[MG], sw[2][2];
+  auto read_x = [&](uint32_t buf, int i) {
+    fx[i] = *reinterpret_cast<const uint4 *>(ring + buf * STAGE + xat + i * 16 * TROW);
+    sx[i] = sring[buf * SST + xsat + i * 64];
+  };
+  auto read_w = [&](uint32_t buf, int q, int j) {
+    fw[q & 1][j] = *reinterpret_cast<const uint4 *>(ring + buf * STAGE + wat + (q * 2 + j) * 16 * TROW);
+    sw[q & 1][j] = sring[buf * SST + wsat + (q * 2 + j) * 64];
+  };
+  auto meet = [&]() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+  };
+
+  mx_f32x4_t acc[MG][8];
+#pragma unroll
+  for (int i = 0; i < MG; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[i][j] = mx_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+  aim();
+  load_stage(); load_stage(); load_stage();
+  __builtin_amdgcn_s_waitcnt(wait_vm(2 * LOADS));              // the first stage
+  meet();
+  uint32_t buf = 0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) read_w(0, 0, j);
+#pragma unroll
+  for (int i = 0; i < MG; ++i) read_x(0, i);
+  bool stored = false;                                         // the tile before sent STORES stores, no more and no fewer
+
+  for (;;) {
+    const At at = locate(tile);
+    OutT bv[8][4];
+    for (int k = 0; k < a.stages; ++k) {
+      // The next stage has landed: at most the loads of the one after it are under way, and at a tile's first two stages the
+      // stores of the tile before, which were sent behind those loads.
+      if (k < 2 && stored) __builtin_amdgcn_s_waitcnt(wait_vm(LOADS + STORES));
+      else __builtin_amdgcn_s_waitcnt(wait_vm(LOADS));
+      meet();
+      load_stage();                                            // into the buffer that the stage before was read from
+      const uint32_t next = (buf + 1) & (TBUF - 1);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+#pragma unroll
+        for (int i = 0; i < MG; ++i) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) mx_mma(acc[i][q * 2 + j], fw[q & 1][j], sw[q & 1][j], fx[i], sx[i]);
+          if (q < 3 && i < 2) read_w(buf, q + 1, i);
+          if (q < 3 && MG == 1) read_w(buf, q + 1, 1);
+          if (q == 3) {
+            if (i < 2) read_w(next, 0, i);
+            if (MG == 1) read_w(next, 0, 1);
+            read_x(next, i);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      buf = next;
+    }
+    // ---- the tile goes out: a lane holds four neighbouring features of token l15 of each group of 16 tokens
+    const int n1 = at.n0 + wn * 128;
+    const bool whole = at.m0 + BM <= a.M && at.n0 + TN <= a.N;
+    OutT *out = pre + (int64_t)at.layer * a.ps + (int64_t)(at.m0 + wm * 16 * MG) * a.pre_row + n1;
+    unsigned char *park = parked + wave * PARK;
+    if (bias) {
+      const OutT *bp = bias + (int64_t)at.layer * a.bs + n1 + lq * 4;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (at.n0 + TN <= a.N) __builtin_memcpy(bv[j], bp + j * 16, 4 * sizeof(OutT));
+        else
+#pragma unroll
+          for (int q = 0; q < 4; ++q) bv[j][q] = bp[min(j * 16 + q, a.N - 1 - n1 - lq * 4)];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < MG; ++i) {
+#pragma unroll
+      for (int h = 0; h < 128 / HF; ++h) {
+#pragma unroll
+        for (int jj = 0; jj < HF / 16; ++jj) {
+          const int j = h * (HF / 16) + jj;
+          float y[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            y[q] = acc[i][j][q] + (bias ? Elem<OutT>::to_f32(bv[j][q]) : 0.0f);
+            acc[i][j][q] = 0.0f;
+          }
+          if constexpr (sizeof(OutT) == 4) {
+            const int slot = (jj * 4 + lq) ^ (l15 & 7);
+            *reinterpret_cast<float4 *>(park + l15 * 128 + slot * 16) = make_float4(y[0], y[1], y[2], y[3]);
+          } else {
+            const int slot = (jj * 2 + (lq >> 1)) ^ (l15 & 7);
+            *reinterpret_cast<uint2 *>(park + l15 * 128 + slot * 16 + (lq & 1) * 8) = make_uint2(pack_pair<OutT>(y[0], y[1]), pack_pair<OutT>(y[2], y[3]));
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          constexpr int PE = 16 / (int)sizeof(OutT);
+          const int row = u * 8 + (lane >> 3), sl = lane & 7;
+          const uint4 v = *reinterpret_cast<const uint4 *>(park + row * 128 + ((sl ^ (row & 7)) * 16));
+          OutT *op = out + (int64_t)(i * 16 + row) * a.pre_row + h * HF + sl * PE;
+          if (whole) {
+            __builtin_memcpy(op, &v, 16);
+          } else if (at.m0 + wm * 16 * MG + i * 16 + row < a.M) {
+            const int left = a.N - (n1 + h * HF + sl * PE);
+            if (left >= PE) __builtin_memcpy(op, &v, 16);
+            else {
+              OutT e[PE];
+              __builtin_memcpy(e, &v, 16);
+#pragma unroll
+              for (int q = 0; q < PE; ++q)
+                if (q < left) op[q] = e[q];
+            }
+          }
+        }
+      }
+    }
+    stored = whole;
+    tile += step;
+    if (tile >= last_tile) break;
+  }
+  __builtin_amdgcn_s_waitcnt(0);   // no load into LDS may be under way when the workgroup ends
+}
+
+// Rows of codes and scales with whole stages of K: the blocks behind the end are zeros.
+__global__ __launch_bounds__(256) void k_mx_widen(const uint8_t *__restrict__ src, uint8_t *__restrict__ dst, int64_t rows, int from, int to,
+                                                  int unit) {
+  const int64_t n = rows * to;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / to;
+    const int b = (int)(i - r * to);
+    if (unit == 16) reinterpret_cast<uint4 *>(dst)[i] = b < from ? reinterpret_cast<const uint4 *>(src)[r * from + b] : make_uint4(0u, 0u, 0u, 0u);
+    else dst[i] = b < from ? src[r * from + b] : (uint8_t)0;
+  }
+}
+
+int launch_mx_widen(const void *src, void *dst, int64_t rows, int64_t from, int64_t to, int unit, hipStream_t s) {
+  const int64_t nb = clt_ceil_div(rows * to, 256);
+  k_mx_widen<<<(unsigned)(nb < 65536 ? nb : 65536), 256, 0, s>>>((const uint8_t *)src, (uint8_t *)dst, rows, (int)from, (int)to, unit);
+  return clt_check_launch();
+}
+
 bool mx_format(int fmt) { return fmt == CLT_MXFP4 || fmt == CLT_MXFP8 || fmt == CLT_MXINT8; }
 uint32_t mx_magic(uint32_t pieces) { return (uint32_t)((0x100000000ull + pieces - 1) / pieces); }
 
 template <typename T, int FMT>
 int launch_mx_write(const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t L, int kinds, int64_t n, int64_t d,
-                    const MxRows &rows, void *codes, uint8_t *scales, hipStream_t s) {
-  const uint32_t blocks = (uint32_t)clt_ceil_div(d, 32), pieces = blocks * 4;
+                    uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, hipStream_t s) {
+  const uint32_t pieces = blocks * 4;
   const int64_t groups = clt_ceil_div(n * (int64_t)pieces, MX_THREADS);
   if (groups > 2147483647LL) return CLT_ERR_RANGE;
   const bool vec = d % 8 == 0 && clt_aligned16(src0) && (kinds == 1 || clt_aligned16(src1)) && (row_stride * (int64_t)sizeof(T)) % 16 == 0 &&
@@ -316,17 +576,17 @@ int launch_mx_write(const void *src0, const void *src1, int64_t layer_stride, in
 
 template <typename T>
 int mx_write_as(int fmt, const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t L, int kinds, int64_t n,
-                int64_t d, const MxRows &rows, void *codes, uint8_t *scales, hipStream_t s) {
-  if (fmt == CLT_MXFP4) return launch_mx_write<T, CLT_MXFP4>(src0, src1, layer_stride, row_stride, L, kinds, n, d, rows, codes, scales, s);
-  if (fmt == CLT_MXFP8) return launch_mx_write<T, CLT_MXFP8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, rows, codes, scales, s);
-  return launch_mx_write<T, CLT_MXINT8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, rows, codes, scales, s);
+                int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, hipStream_t s) {
+  if (fmt == CLT_MXFP4) return launch_mx_write<T, CLT_MXFP4>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
+  if (fmt == CLT_MXFP8) return launch_mx_write<T, CLT_MXFP8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
+  return launch_mx_write<T, CLT_MXINT8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
 }
 
 int mx_write(int dtype, int fmt, const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t L, int kinds,
-             int64_t n, int64_t d, const MxRows &rows, void *codes, uint8_t *scales, hipStream_t s) {
-  if (dtype == CLT_BF16) return mx_write_as<bf16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, rows, codes, scales, s);
-  if (dtype == CLT_F16) return mx_write_as<f16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, rows, codes, scales, s);
-  return mx_write_as<float>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, rows, codes, scales, s);
+             int64_t n, int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, hipStream_t s) {
+  if (dtype == CLT_BF16) return mx_write_as<bf16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
+  if (dtype == CLT_F16) return mx_write_as<f16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
+  return mx_write_as<float>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
 }
 
 template <typename OutT, int FMT>
@@ -363,14 +623,54 @@ int mx_read(int dtype, int fmt, const void *codes, const uint8_t *scales, const 
   return mx_read_as<float>(fmt, codes, scales, rows, L, kinds, n, d, nm, out0, out1, out_layer_stride, out_row_stride, s);
 }
 
+// Batches that the tile kernel takes, in tokens.
+constexpr int64_t MX_TILE_MIN_TOKENS = 129;
+
+// What the projection keeps for itself: x in codes, rows of whole stages; the scales of W where their rows are not.
+struct MxPlan {
+  int64_t blocks, padded;      // blocks of a row, and in whole stages
+  bool tiles;
+  size_t xc, xs, ws, bytes;    // offsets in the workspace
+};
+MxPlan mx_plan(int64_t T, int64_t d, int64_t F, int64_t L, bool quantised) {
+  MxPlan p{};
+  p.blocks = clt_ceil_div(d, 32);
+  p.tiles = T >= MX_TILE_MIN_TOKENS;
+  p.padded = p.tiles ? (p.blocks + 3) / 4 * 4 : p.blocks;
+  const bool own_x = !quantised || p.padded != p.blocks;
+  auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+  p.xs = up(own_x ? (size_t)(L * T * p.padded * 16) : 0);
+  p.ws = p.xs + up(own_x ? (size_t)(L * T * p.padded) : 0);
+  p.bytes = p.ws + up(p.padded != p.blocks ? (size_t)(L * F * p.padded) : 0);
+  return p;
+}
+
+// One persistent workgroup per CU, a whole number of rounds over the 8 XCDs; 0 when the device cannot be asked.
+int mx_grid(int64_t tiles) {
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 8) return 0;
+  const int64_t per = clt_ceil_div(tiles, 8);
+  return (int)(per * 8 < cus - cus % 8 ? per * 8 : cus - cus % 8);
+}
+
 template <typename OutT>
-int launch_mx_project(const uint8_t *xc, const uint8_t *xs, const uint8_t *wc, const uint8_t *wsc, const void *bias, void *pre, int64_t T,
-                      int64_t d, int64_t F, int64_t L, int64_t bs, int64_t ps, int64_t pre_row, hipStream_t s) {
-  const int blocks = (int)clt_ceil_div(d, 32);
+int launch_mx_project(const MxPlan &p, const uint8_t *xc, const uint8_t *xs, const uint8_t *wc, const uint8_t *wsc, const void *bias, void *pre,
+                      int64_t T, int64_t F, int64_t L, int64_t bs, int64_t ps, int64_t pre_row, hipStream_t s) {
+  if (p.tiles) {
+    constexpr int MG = 4;
+    const int64_t tm = clt_ceil_div(T, 64 * MG), tn = clt_ceil_div(F, TN), total = tm * tn * L;
+    if (total > 1073741824LL) return CLT_ERR_RANGE;
+    const int grid = mx_grid(total);
+    if (grid <= 0) return CLT_ERR_LAUNCH;
+    TileArgs a{xc, xs, wc, wsc, (int)T, (int)F, (int)tm, (int)tn, (int)total, (int)clt_ceil_div(total, 8), (int)(p.padded / 4),
+               (int)p.padded * 16, (int)p.blocks * 16, (int)p.padded, (int)p.blocks, bs, ps, pre_row};
+    k_mx_project_tiles<OutT, MG><<<grid, TW * 64, 0, s>>>(a, (const OutT *)bias, (OutT *)pre);
+    return clt_check_launch();
+  }
+  const int blocks = (int)p.blocks;
 #define CLT_MXP(NF, MT)                                                                                                          \
   {                                                                                                                              \
     const dim3 grid((unsigned)clt_ceil_div(F, 64 * NF), (unsigned)clt_ceil_div(T, 16 * MT), (unsigned)L);                          \
-    if (grid.y > 65535u) return CLT_ERR_RANGE;                                                                                   \
     k_mx_project<OutT, NF, MT><<<grid, 256, 0, s>>>(xc, xs, wc, wsc, (const OutT *)bias, (OutT *)pre, (int)T, (int)F, blocks, bs, ps, pre_row); \
   }
   if (T <= 16) CLT_MXP(2, 1)
@@ -402,7 +702,7 @@ extern "C" int clt_mx_quantise(const void *src, int64_t n, int64_t d, int64_t ro
   if (!src || !codes || !scales || (n > 1 && row_stride < d)) return CLT_ERR_ARG;
   if (!clt_aligned16(codes)) return CLT_ERR_ALIGN;
   const MxRows rows{nullptr, 0, 0, n, nullptr};
-  return mx_write(dtype, fmt, src, nullptr, 0, row_stride, 1, 1, n, d, rows, codes, scales, (hipStream_t)stream);
+  return mx_write(dtype, fmt, src, nullptr, 0, row_stride, 1, 1, n, d, (uint32_t)clt_ceil_div(d, 32), rows, codes, scales, (hipStream_t)stream);
 }
 
 extern "C" int clt_mx_dequantise(const void *codes, const uint8_t *scales, int64_t n, int64_t d, int fmt, void *dst, int64_t row_stride,
@@ -435,7 +735,7 @@ extern "C" int clt_mx_cache_write(const void *x, const void *tgt, int64_t layer_
     k_mx_claim<<<nb, 256, 0, s>>>(r, n, owner, 0);
     k_mx_claim<<<nb, 256, 0, s>>>(r, n, owner, 1);
   }
-  return mx_write(dtype, fmt, x, tgt, layer_stride, row_stride, L, 2, n, d, r, codes, scales, s);
+  return mx_write(dtype, fmt, x, tgt, layer_stride, row_stride, L, 2, n, d, (uint32_t)clt_ceil_div(d, 32), r, codes, scales, s);
 }
 
 extern "C" int clt_mx_cache_read(const void *codes, const uint8_t *scales, int64_t rows, int fmt, const void *row_index, int index_bits,
@@ -458,18 +758,46 @@ extern "C" int clt_mx_cache_read(const void *codes, const uint8_t *scales, int64
                  (hipStream_t)stream);
 }
 
-extern "C" int clt_mx_encode(const void *x_codes, const uint8_t *x_scales, const void *w_codes, const uint8_t *w_scales, const void *bias,
-                             void *pre, int64_t T, int64_t d, int64_t F, int64_t L, int64_t b_layer_stride, int64_t pre_layer_stride,
-                             int64_t pre_row_stride, int dtype, void *stream) {
+extern "C" size_t clt_mx_encode_workspace_bytes(int64_t T, int64_t d, int64_t F, int64_t L, int x_quantised) {
+  if (T <= 0 || d <= 0 || F <= 0 || L <= 0 || d > MX_MAX_WIDTH) return 0;
+  return mx_plan(T, d, F, L, x_quantised != 0).bytes;
+}
+
+extern "C" int clt_mx_encode(const void *x, const uint8_t *x_scales, const void *w_codes, const uint8_t *w_scales, const void *bias, void *pre,
+                             int64_t T, int64_t d, int64_t F, int64_t L, int64_t x_layer_stride, int64_t b_layer_stride,
+                             int64_t pre_layer_stride, int64_t pre_row_stride, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
   if (!clt_model_dtype(dtype)) return CLT_ERR_DTYPE;
   if (T < 0 || d <= 0 || F <= 0 || L <= 0) return CLT_ERR_ARG;
   if (T == 0) return CLT_OK;
-  if (!x_codes || !x_scales || !w_codes || !w_scales || !pre || pre_row_stride < F || pre_layer_stride < 0) return CLT_ERR_ARG;
-  if (d > MX_MAX_WIDTH || T > (1 << 20) || F > (1 << 30) || L > 65535) return CLT_ERR_RANGE;
-  if (!clt_aligned16(x_codes) || !clt_aligned16(w_codes)) return CLT_ERR_ALIGN;
+  if (!x || !w_codes || !w_scales || !pre || pre_row_stride < F || pre_layer_stride < 0 || (!x_scales && x_layer_stride < 0)) return CLT_ERR_ARG;
+  if (d > MX_MAX_WIDTH || T > (1 << 20) || F > (1 << 30) || L > 32767) return CLT_ERR_RANGE;
+  if ((x_scales && !clt_aligned16(x)) || !clt_aligned16(w_codes)) return CLT_ERR_ALIGN;
+  const MxPlan p = mx_plan(T, d, F, L, x_scales != nullptr);
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return CLT_ERR_WORKSPACE;
+  if (p.bytes > 0 && !clt_aligned16(workspace)) return CLT_ERR_ALIGN;
+  // the tile kernel fetches four scales at a time
+  if (p.tiles && p.padded == p.blocks && (((uintptr_t)w_scales | (uintptr_t)x_scales) & 3u) != 0) return CLT_ERR_ALIGN;
   hipStream_t s = (hipStream_t)stream;
-  const uint8_t *xc = (const uint8_t *)x_codes, *wc = (const uint8_t *)w_codes;
-  if (dtype == CLT_BF16) return launch_mx_project<bf16_t>(xc, x_scales, wc, w_scales, bias, pre, T, d, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s);
-  if (dtype == CLT_F16) return launch_mx_project<f16_t>(xc, x_scales, wc, w_scales, bias, pre, T, d, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s);
-  return launch_mx_project<float>(xc, x_scales, wc, w_scales, bias, pre, T, d, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s);
+  uint8_t *ws = (uint8_t *)workspace;
+  const uint8_t *xc = (const uint8_t *)x, *xs = x_scales, *wc = (const uint8_t *)w_codes, *wsc = w_scales;
+  int rc = CLT_OK;
+  if (!x_scales) {
+    const MxRows rows{nullptr, 0, 0, T, nullptr};
+    rc = mx_write(dtype, CLT_MXFP4, x, nullptr, x_layer_stride, d, L, 1, T, d, (uint32_t)p.padded, rows, ws + p.xc, ws + p.xs, s);
+    xc = ws + p.xc;
+    xs = ws + p.xs;
+  } else if (p.padded != p.blocks) {
+    rc = launch_mx_widen(x, ws + p.xc, L * T, p.blocks, p.padded, 16, s);
+    if (rc == CLT_OK) rc = launch_mx_widen(x_scales, ws + p.xs, L * T, p.blocks, p.padded, 1, s);
+    xc = ws + p.xc;
+    xs = ws + p.xs;
+  }
+  if (rc == CLT_OK && p.padded != p.blocks) {
+    rc = launch_mx_widen(w_scales, ws + p.ws, L * F, p.blocks, p.padded, 1, s);
+    wsc = ws + p.ws;
+  }
+  if (rc != CLT_OK) return rc;
+  if (dtype == CLT_BF16) return launch_mx_project<bf16_t>(p, xc, xs, wc, wsc, bias, pre, T, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s);
+  if (dtype == CLT_F16) return launch_mx_project<f16_t>(p, xc, xs, wc, wsc, bias, pre, T, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s);
+  return launch_mx_project<float>(p, xc, xs, wc, wsc, bias, pre, T, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s);
 }

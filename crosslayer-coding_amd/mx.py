@@ -82,6 +82,8 @@ class MXTensor:
                              "do not belong together")
         if codes.data_ptr() % 16 != 0:
             raise ValueError("codes must begin at a multiple of 16 bytes")
+        if scales.data_ptr() % 4 != 0:
+            scales = scales.clone()                 # the kernels fetch four at a time
         self.codes, self.scales, self.fmt, self.width = codes, scales, fmt, int(width)
 
     @property
@@ -143,10 +145,11 @@ def quantise(x: torch.Tensor, fmt: str = "mxfp4", out: Optional[MXTensor] = None
 
 
 def project(x: Union[torch.Tensor, MXTensor], w: MXTensor, b: Optional[torch.Tensor] = None,
-            out: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+            out: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None, ws=None) -> torch.Tensor:
     """``pre[l] = x[l] @ w[l].T + b[l]`` on the 4-bit matrix cores: ``w`` [L, F, d] in mxfp4, ``x`` [L, T, d] quantised to
     mxfp4 on the way in (or an `MXTensor` that is), fp32 sums, one rounding.  ``b`` [L, F]; [T, d] with w [F, d] and b [F]
-    is one layer.  The result has x's type, or ``out``'s / b's / ``dtype`` where x comes quantised."""
+    is one layer.  The result has x's type, or ``out``'s / b's / ``dtype`` where x comes quantised.  ``ws``: an
+    `engine.Workspace` to take the scratch memory from."""
     if w.fmt != "mxfp4" or len(w.shape) not in (2, 3):
         raise ValueError(f"the weights must be mxfp4 [L, F, d] or [F, d], got {w.fmt} {tuple(w.shape)}")
     if len(x.shape) != len(w.shape) or x.shape[-1] != w.width or x.shape[:-2] != w.shape[:-2]:
@@ -176,15 +179,23 @@ def project(x: Union[torch.Tensor, MXTensor], w: MXTensor, b: Optional[torch.Ten
         raise ValueError(f"out must be contiguous {dtype} {shape} on {w.device}")
     if out.numel() == 0:
         return out
-    xq = x if isinstance(x, MXTensor) else quantise(x, "mxfp4")
     if b is not None and not b.is_contiguous():
         b = b.contiguous()
+    given = isinstance(x, MXTensor)
+    if not given:
+        x = x.contiguous()
     T, F = shape[-2], shape[-1]
     L = shape[0] if len(shape) == 3 else 1
+    lib = nat.load()
     with torch.cuda.device(w.device):
-        code = nat.load().clt_mx_encode(nat.ptr(xq.codes), nat.ptr(xq.scales), nat.ptr(w.codes), nat.ptr(w.scales), nat.ptr(b),
-                                        nat.ptr(out), T, w.width, F, L, F, T * F, F, nat.dtype_code(dtype),
-                                        nat.current_stream(w.device))
+        nbytes = lib.clt_mx_encode_workspace_bytes(T, w.width, F, L, int(given))
+        if ws is not None:
+            scratch = ws.get("mx_project", nbytes)
+        else:
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
+        code = lib.clt_mx_encode(nat.ptr(x.codes if given else x), nat.ptr(x.scales if given else None), nat.ptr(w.codes), nat.ptr(w.scales),
+                                 nat.ptr(b), nat.ptr(out), T, w.width, F, L, T * w.width, F, T * F, F, nat.dtype_code(dtype),
+                                 nat.ptr(scratch), scratch.numel(), nat.current_stream(w.device))
     nat.check(code, "clt_mx_encode")
     return out
 

@@ -904,10 +904,12 @@ int clt_feed_gather(const void *src, int src_dtype, int64_t src_rows, int64_t sr
  *   read: rows [out_row0, out_row0 + n) of x_out, tgt_out [L][T][d] (out_dtype) from rows row_index[j] or first + j;
  *     normalisation and arguments as in clt_feed_gather.  A row number outside [0, rows) is not read: its row is NaN.
  *
- * clt_mx_encode: pre[l] = x[l] . w[l]^T + b[l] with both operands in CLT_MXFP4 (x [L][T], w [L][F] rows of d elements):
- *   exact products, fp32 sums, the bias added in fp32, one rounding to dtype (that of bias and pre; bias may be NULL).
- *   pre rows are pre_row_stride >= F elements apart.  What clt_encode computes from 16- or 32-bit operands
- *   (clt/models/parallel.py:286).  T up to 2^20, F up to 2^30, L up to 65535.
+ * clt_mx_encode: pre[l] = x[l] . w[l]^T + b[l] with both operands in CLT_MXFP4: exact products, fp32 sums, the bias
+ *   added in fp32, one rounding to dtype (that of bias and pre; bias may be NULL).  w [L][F] rows of d elements.  x is
+ *   [L][T][d] values of dtype, layers x_layer_stride apart, which the call quantises, when x_scales is NULL; else its
+ *   codes and scales [L][T].  pre rows are pre_row_stride >= F elements apart, layers pre_layer_stride.
+ *   What clt_encode computes from 16- or 32-bit operands (clt/models/parallel.py:286).  workspace: 16-byte aligned,
+ *   clt_mx_encode_workspace_bytes (may be 0 when x comes quantised).  Scales begin 4-byte aligned.  T up to 2^20, F up to 2^30, L up to 32767.
  */
 #define CLT_MXFP4 0
 #define CLT_MXFP8 1
@@ -927,10 +929,12 @@ int clt_mx_cache_read(const void *codes, const uint8_t *scales, int64_t rows, in
                       int64_t L, int norm_mode, const float *mean_in, const float *std_in,
                       const float *mean_tg, const float *std_tg, double scale, void *x_out,
                       void *tgt_out, int64_t out_row0, int64_t T, int out_dtype, void *stream);
-int clt_mx_encode(const void *x_codes, const uint8_t *x_scales, const void *w_codes,
+size_t clt_mx_encode_workspace_bytes(int64_t T, int64_t d, int64_t F, int64_t L, int x_quantised);
+int clt_mx_encode(const void *x, const uint8_t *x_scales, const void *w_codes,
                   const uint8_t *w_scales, const void *bias, void *pre, int64_t T, int64_t d,
-                  int64_t F, int64_t L, int64_t b_layer_stride, int64_t pre_layer_stride,
-                  int64_t pre_row_stride, int dtype, void *stream);
+                  int64_t F, int64_t L, int64_t x_layer_stride, int64_t b_layer_stride,
+                  int64_t pre_layer_stride, int64_t pre_row_stride, int dtype, void *workspace,
+                  size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
