@@ -53,6 +53,15 @@ template <int FMT> __device__ __forceinline__ uint2 mx_encode8(const float (&v)[
 }
 
 typedef __attribute__((ext_vector_type(2))) float mx_f32x2_t;
+typedef __attribute__((ext_vector_type(2))) __bf16 mx_bf16x2_t;
+typedef __attribute__((ext_vector_type(2))) _Float16 mx_f16x2_t;
+
+// two floats as packed 16-bit elements, rounded to nearest even
+template <typename T> __device__ __forceinline__ uint32_t mx_pack(float a, float b) {
+  const mx_f32x2_t v = {a, b};
+  if constexpr (IsHalf<T>::value) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, mx_f16x2_t));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, mx_bf16x2_t));
+}
 
 // The values eight codes stand for, before the block's scale.
 template <int FMT> __device__ __forceinline__ void mx_decode8(const uint2 &c, float (&v)[8]) {
@@ -214,8 +223,8 @@ __global__ __launch_bounds__(MX_THREADS) void k_mx_read(const uint8_t *__restric
   OutT *op = (kind ? out1 : out0) + l * out_layer_stride + at.j * out_row_stride + c;
   if constexpr (VEC) {
     if constexpr (sizeof(OutT) == 2) {
-      *reinterpret_cast<uint4 *>(op) = make_uint4(pack_pair<OutT>(v[0], v[1]), pack_pair<OutT>(v[2], v[3]), pack_pair<OutT>(v[4], v[5]),
-                                                  pack_pair<OutT>(v[6], v[7]));
+      *reinterpret_cast<uint4 *>(op) = make_uint4(mx_pack<OutT>(v[0], v[1]), mx_pack<OutT>(v[2], v[3]), mx_pack<OutT>(v[4], v[5]),
+                                                  mx_pack<OutT>(v[6], v[7]));
     } else {
       *reinterpret_cast<float4 *>(op) = make_float4(v[0], v[1], v[2], v[3]);
       *reinterpret_cast<float4 *>(op + 4) = make_float4(v[4], v[5], v[6], v[7]);
@@ -236,6 +245,13 @@ typedef __attribute__((ext_vector_type(4))) float mx_f32x4_t;
 __device__ __forceinline__ void mx_mma(mx_f32x4_t &acc, const uint4 &a, uint32_t sa, const uint4 &b, uint32_t sb) {
   const mx_i32x8_t av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0}, bv = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
   acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc, 4, 4, 0, (int)sa, 0, (int)sb);
+}
+
+// The same with the scale in byte ks of the word.
+__device__ __forceinline__ void mx_mma2(mx_f32x4_t &acc, const uint4 &a, uint32_t sa, const uint4 &b, uint32_t sb, int ks) {
+  const mx_i32x8_t av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0}, bv = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
+  if (ks == 0) acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc, 4, 4, 0, (int)sa, 0, (int)sb);
+  else acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc, 4, 4, 1, (int)sa, 1, (int)sb);
 }
 
 // pre[l][m][n] = b[l][n] + sum over k of x[l][m][k] w[l][n][k].  A wavefront takes 16 NF features x 16 MT tokens, its operands
@@ -296,18 +312,23 @@ __global__ __launch_bounds__(256) void k_mx_project(const uint8_t *__restrict__ 
 
 // ---- the projection of a batch ------------------------------------------------------------------------------------
 // Tiles of BM tokens x 256 features, one persistent workgroup of 8 wavefronts (4 along the tokens, 2 along the features) per CU.
-// A stage is 128 elements of K: 64 bytes of codes and 4 of scales per row, brought straight into one of four buffers in
-// LDS, chunk c of row r at chunk position c ^ ((r >> 2) & 3), so that the 16 rows of a fragment read lie in all banks.  The
-// stages of all of a workgroup's tiles form one sequence: at the barrier in front of a stage the next one has landed too,
-// and the third after it is asked for, so a load has two stages to arrive, the fragments of the next stage are read under
-// the products of this one, and the first stages of the next tile travel during the last ones of this tile.
+// A stage is 256 elements of K: 128 bytes of codes per row - whole cache lines - and 8 of scales, brought straight into
+// LDS, chunk c of row r at chunk position c ^ ((r >> 1) & 7), so that the 16 rows of a fragment read lie in all banks.  A lane
+// multiplies the blocks 2 lq and 2 lq + 1 of its row (lq = lane / 16): their scales are neighbours and come in one read.
+//
+// A stage is four quarters of 4 MG products: all tokens of the wavefront x 32 of its features.  The x fragments stay in
+// registers for the stage, each being replaced by the next stage's behind its last use; the W fragments of the next quarter are
+// read under this one's products.  Two barriers: at the first, behind quarter 0, x and the first half of W have been read by
+// everybody, so those loads of the stage after next (and its scales, which have three places) are asked for; at the second,
+// behind quarter 2, the rest.  A load has a stage and a half to arrive.  The stages of all of a workgroup's tiles form one
+// sequence: the first stages of the next tile travel during the last ones of this tile, and its stores during the next.
 constexpr int TN = 256;                       // features of a tile
 constexpr int TW = 8;                         // wavefronts
-constexpr int TROW = 64;                      // bytes of codes per row and stage
-constexpr int TBUF = 4;
+constexpr int TROW = 128;                     // bytes of codes per row and stage
+constexpr int TBLOCKS = 8;                    // blocks per row and stage
 constexpr int PARK = 2048;                    // bytes of a wavefront's piece of the output tile on its way out
 
-// vmcnt(n), everything else unconstrained
+// vmcnt(n), nothing asked of the other counters
 constexpr int wait_vm(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0F70; }
 
 __device__ __forceinline__ uint32_t mx_lds(const void *p) {
@@ -323,9 +344,9 @@ __device__ __forceinline__ void mx_fill4(const void *base, uint32_t off, uint32_
 }
 
 struct TileArgs {
-  const uint8_t *xc, *xs, *wc, *ws;           // x rows hold whole stages (zeros behind the end), so do all scale rows
+  const uint8_t *xc, *xs, *wc, *ws;           // x rows, codes and scales, hold whole stages (zeros behind the end)
   int M, N, tiles_m, tiles_n, total, per_xcd;
-  int stages, xpitch, wpitch, spitch, wblocks;   // bytes of a row of codes, of scales; blocks of W that are there
+  int stages, xpitch, wpitch, xspitch, wspitch;   // bytes of a row of codes, of scales
   int64_t bs, ps, pre_row;
 };
 
@@ -333,16 +354,18 @@ template <typename OutT, int MG>
 __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_mx_project_tiles(
     TileArgs a, const OutT *__restrict__ bias, OutT *__restrict__ pre) {
   constexpr int BM = 64 * MG;                              // tokens of a tile; a wavefront takes 16 MG x 128
-  constexpr int XI = BM / 16, XPW = XI >= TW ? XI / TW : 1;   // loads of 16 rows of x; per wavefront (some twice where there are few)
-  constexpr int SI = (BM + TN) / 64;                       // loads of the scales of 64 rows
-  constexpr int LOADS = XPW + 2 + 1;                       // of a stage, per wavefront
-  constexpr int STAGE = (BM + TN) * TROW, SST = (BM + TN) * 4;
+  constexpr int SI = (BM + TN) / 32;                       // loads of the scales of 32 rows
+  constexpr int FIRST = MG + 2 + 2, REST = 2;              // loads of a stage per wavefront: x, first half of W, scales; rest of W
+  constexpr int LOADS = FIRST + REST;
+  constexpr int STAGE = (BM + TN) * TROW, SST = (BM + TN) * TBLOCKS;
   constexpr int HF = 128 / (int)sizeof(OutT);              // features of a parked piece: rows of 128 bytes
   constexpr int STORES = MG * (128 / HF) * 2;              // stores of a whole tile, per wavefront
+  constexpr int G = 2 * MG;                                // pairs of products per quarter
   static_assert(LOADS + STORES < 64, "the wait counter holds 63");
-  __shared__ __attribute__((aligned(16))) unsigned char ring[TBUF * STAGE];
-  __shared__ __attribute__((aligned(16))) unsigned char sring[TBUF * SST];
+  __shared__ __attribute__((aligned(16))) unsigned char ring[2 * STAGE];
+  __shared__ __attribute__((aligned(16))) unsigned char sring[3 * SST];
   __shared__ __attribute__((aligned(16))) unsigned char parked[TW * PARK];
+  __shared__ __attribute__((aligned(16))) float bias_lds[TW][128];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave & 3, wn = wave >> 2, l15 = lane & 15, lq = lane >> 4;
   const uint32_t ring0 = mx_lds(ring), sring0 = mx_lds(sring);
@@ -367,55 +390,76 @@ __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   int tile = ((int)blockIdx.x & 7) * a.per_xcd + ((int)blockIdx.x >> 3);
   if (tile >= last_tile) return;
 
-  // ---- the loader: where its next stage comes from
+  // ---- the loader: where its next stage comes from.  A load of codes brings 8 rows, lane l row l / 8 at chunk position l % 8.
   int in_tile = tile, in_stage = 0;
-  uint32_t in_buf = 0, xo[XPW], wo[2], so;
-  const uint8_t *in_x, *in_w, *in_s;
-  const uint32_t chunk = (uint32_t)((lane & 3) ^ ((lane >> 4) & 3));
-  const int sunit = wave % SI;
+  uint32_t in_buf = 0, in_sbuf = 0, xo[MG], wo[4], so[2];
+  const uint8_t *in_x, *in_w, *in_s[2];
+  const uint32_t chunkE = (uint32_t)((lane & 7) ^ (lane >> 4)) * 16u;      // groups of 8 rows that begin at 0 mod 16; at 8: ^ 64
+  // x: rows 8 MG wave + 8 i.  W: row groups in the order of the quarters, first half 0 .. 63 and 128 .. 191, rest behind them
+  auto w_row = [&](int i) { const int u = (i & 1) * 8 + wave; return (i >> 1) * 64 + (u >> 3) * 128 + (u & 7) * 8; };
   auto aim = [&]() {
     const At at = locate(in_tile);
+    int la = lane;                                            // rebuilt for every tile, see the epilogue
+    asm volatile("" : "+v"(la));
+    const int lr = la >> 3;
     in_x = a.xc + ((int64_t)at.layer * a.M + at.m0) * a.xpitch;
     in_w = a.wc + ((int64_t)at.layer * a.N + at.n0) * a.wpitch;
     const int xl = a.M - 1 - at.m0, wl = a.N - 1 - at.n0;     // rows past the end repeat the last one
 #pragma unroll
-    for (int i = 0; i < XPW; ++i) xo[i] = (uint32_t)min(((wave * XPW + i) % XI) * 16 + (lane >> 2), xl) * (uint32_t)a.xpitch + chunk * 16u;
+    for (int i = 0; i < MG; ++i) {
+      const int r = (wave * MG + i) * 8;
+      xo[i] = (uint32_t)min(r + lr, xl) * (uint32_t)a.xpitch + (chunkE ^ ((r & 8) ? 64u : 0u));
+    }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) wo[i] = (uint32_t)min((wave * 2 + i) * 16 + (lane >> 2), wl) * (uint32_t)a.wpitch;
-    const bool of_x = sunit * 64 < BM;
-    in_s = of_x ? a.xs + ((int64_t)at.layer * a.M + at.m0) * a.spitch : a.ws + ((int64_t)at.layer * a.N + at.n0) * a.spitch;
-    so = (uint32_t)min((of_x ? sunit * 64 : sunit * 64 - BM) + lane, of_x ? xl : wl) * (uint32_t)a.spitch;
-  };
-  auto load_stage = [&]() {
-    const uint32_t at = ring0 + in_buf * STAGE, sat = sring0 + in_buf * SST;
+    for (int i = 0; i < 4; ++i) wo[i] = (uint32_t)min(w_row(i) + lr, wl) * (uint32_t)a.wpitch;
 #pragma unroll
-    for (int i = 0; i < XPW; ++i) mx_fill16(in_x + (int64_t)in_stage * TROW, xo[i], at + (uint32_t)((wave * XPW + i) % XI) * 1024u);
-    const uint32_t k16 = (uint32_t)min(in_stage * 4 + (int)chunk, a.wblocks - 1) * 16u;   // x is zero where W repeats its last block
-#pragma unroll
-    for (int i = 0; i < 2; ++i) mx_fill16(in_w, wo[i] + k16, at + BM * TROW + (uint32_t)(wave * 2 + i) * 1024u);
-    mx_fill4(in_s + (int64_t)in_stage * 4, so, sat + (uint32_t)sunit * 256u);
-    in_buf = (in_buf + 1) & (TBUF - 1);
-    if (++in_stage == a.stages) {
-      in_stage = 0;
-      if (in_tile + step < last_tile) in_tile += step;         // behind the last tile: once more, for nobody
-      aim();
+    for (int i = 0; i < 2; ++i) {
+      const int r = (wave * 2 + i) % SI * 32;
+      const bool of_x = r < BM;
+      in_s[i] = of_x ? a.xs + ((int64_t)at.layer * a.M + at.m0) * a.xspitch : a.ws + ((int64_t)at.layer * a.N + at.n0) * a.wspitch;
+      so[i] = (uint32_t)min((of_x ? r : r - BM) + (la >> 1), of_x ? xl : wl) * (uint32_t)(of_x ? a.xspitch : a.wspitch);
     }
   };
+  // W and its scales are not filled up: behind the end the last block is repeated, and x is zero there
+  auto load_w = [&](int i) {
+    const int r = w_row(i);
+    mx_fill16(in_w, wo[i] + min((uint32_t)in_stage * TROW + (chunkE ^ ((r & 8) ? 64u : 0u)), (uint32_t)a.wpitch - 16u), ring0 + in_buf * STAGE + (uint32_t)(BM + r) * TROW);
+  };
+  auto load_first = [&](int i) {
+    if (i < MG) mx_fill16(in_x + (int64_t)in_stage * TROW, xo[i], ring0 + in_buf * STAGE + (uint32_t)(wave * MG + i) * (8 * TROW));
+    else if (i < MG + 2) load_w(i - MG);
+    else {
+      const int u = (wave * 2 + i - MG - 2) % SI;
+      const uint32_t pitch = (uint32_t)(u * 32 < BM ? a.xspitch : a.wspitch);
+      mx_fill4(in_s[i - MG - 2], so[i - MG - 2] + min((uint32_t)in_stage * 8u + (uint32_t)(lane & 1) * 4u, pitch - 4u),
+               sring0 + in_sbuf * SST + (uint32_t)u * 256u);
+    }
+  };
+  auto load_rest = [&](int i) { load_w(2 + i); };
+  auto load_next = [&]() {
+    in_buf ^= 1u;
+    in_sbuf = in_sbuf == 2 ? 0 : in_sbuf + 1;
+    ++in_stage;
+  };
+  auto load_from = [&]() {                                     // in front of a stage's first load
+    if (in_stage != a.stages) return;
+    in_stage = 0;
+    if (in_tile + step < last_tile) in_tile += step;           // behind the last tile: once more, for nobody
+    aim();
+  };
 
-  // ---- fragments: row l15 of each group of 16, its block lq
-  const uint32_t pos = (uint32_t)(lq ^ (l15 >> 2)) * 16u;
-  const uint32_t xat = (uint32_t)(wm * 16 * MG + l15) * TROW + pos, wat = (uint32_t)(BM + wn * 128 + l15) * TROW + pos;
-  const uint32_t xsat = (uint32_t)(wm * 16 * MG + l15) * 4 + lq, wsat = (uint32_t)(BM + wn * 128 + l15) * 4 + lq;
-  uint4 fx[MG], fw[2][2];
+  // ---- fragments: row l15 of each group of 16, its blocks 2 lq and 2 lq + 1
+  const uint32_t xat = (uint32_t)(wm * 16 * MG + l15) * TROW, wat = (uint32_t)(BM + wn * 128 + l15) * TROW;
+  const uint32_t xsat = (uint32_t)(wm * 16 * MG + l15) * TBLOCKS + lq * 2, wsat = (uint32_t)(BM + wn * 128 + l15) * TBLOCKS + lq * 2;
+  const uint32_t koff[2] = {(uint32_t)((lq * 2) ^ ((l15 >> 1) & 7)) * 16u, (uint32_t)((lq * 2 + 1) ^ ((l15 >> 1) & 7)) * 16u};
+  uint4 fx[MG][2], fw[2][2][2];
   uint32_t sx[MG], sw[2][2];
-  auto read_x = [&](uint32_t buf, int i) {
-    fx[i] = *reinterpret_cast<const uint4 *>(ring + buf * STAGE + xat + i * 16 * TROW);
-    sx[i] = sring[buf * SST + xsat + i * 64];
+  auto read_x = [&](uint32_t buf, int i, int ks) { fx[i][ks] = *reinterpret_cast<const uint4 *>(ring + buf * STAGE + xat + i * 16 * TROW + koff[ks]); };
+  auto read_xs = [&](uint32_t sbuf, int i) { sx[i] = *reinterpret_cast<const uint16_t *>(sring + sbuf * SST + xsat + i * 16 * TBLOCKS); };
+  auto read_w = [&](uint32_t buf, int q, int j, int ks) {
+    fw[q & 1][j][ks] = *reinterpret_cast<const uint4 *>(ring + buf * STAGE + wat + (q * 2 + j) * 16 * TROW + koff[ks]);
   };
-  auto read_w = [&](uint32_t buf, int q, int j) {
-    fw[q & 1][j] = *reinterpret_cast<const uint4 *>(ring + buf * STAGE + wat + (q * 2 + j) * 16 * TROW);
-    sw[q & 1][j] = sring[buf * SST + wsat + (q * 2 + j) * 64];
-  };
+  auto read_ws = [&](uint32_t sbuf, int q, int j) { sw[q & 1][j] = *reinterpret_cast<const uint16_t *>(sring + sbuf * SST + wsat + (q * 2 + j) * 16 * TBLOCKS); };
   auto meet = [&]() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -430,105 +474,150 @@ __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[i][j] = mx_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
+  // The bias of a tile, two features per lane: asked for in front of the stores of the tile before, so that its arrival does not
+  // wait for them, and put into LDS behind them.
+  float b0 = 0.0f, b1 = 0.0f;
+  auto load_bias = [&](int t) {
+    if (!bias) return;
+    const At at = locate(t);
+    int la = lane;
+    asm volatile("" : "+v"(la));
+    const OutT *bp = bias + (int64_t)at.layer * a.bs;
+    const int n = at.n0 + wn * 128 + la * 2;
+    b0 = Elem<OutT>::to_f32(bp[min(n, a.N - 1)]);
+    b1 = Elem<OutT>::to_f32(bp[min(n + 1, a.N - 1)]);
+  };
+  auto keep_bias = [&]() { *reinterpret_cast<float2 *>(&bias_lds[wave][lane * 2]) = make_float2(b0, b1); };
+
+  load_bias(tile);
+  keep_bias();
   aim();
-  load_stage(); load_stage(); load_stage();
-  __builtin_amdgcn_s_waitcnt(wait_vm(2 * LOADS));              // the first stage
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    load_from();
+#pragma unroll
+    for (int i = 0; i < FIRST; ++i) load_first(i);
+#pragma unroll
+    for (int i = 0; i < REST; ++i) load_rest(i);
+    load_next();
+  }
+  __builtin_amdgcn_s_waitcnt(wait_vm(LOADS));                  // the first stage
   meet();
-  uint32_t buf = 0;
+  uint32_t buf = 0, sbuf = 0;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) read_w(0, 0, j);
+  for (int j = 0; j < 2; ++j) {
+    read_ws(0, 0, j);
 #pragma unroll
-  for (int i = 0; i < MG; ++i) read_x(0, i);
-  bool stored = false;                                         // the tile before sent STORES stores, no more and no fewer
+    for (int ks = 0; ks < 2; ++ks) read_w(0, 0, j, ks);
+  }
+#pragma unroll
+  for (int i = 0; i < MG; ++i) {
+    read_xs(0, i);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) read_x(0, i, ks);
+  }
+  // barriers still to come at which the stores of the tile before are allowed for: STORES of them, no more and no fewer, were
+  // sent behind what these wait for
+  int behind = 0;
 
   for (;;) {
     const At at = locate(tile);
-    OutT bv[8][4];
+#pragma clang loop unroll(disable)
     for (int k = 0; k < a.stages; ++k) {
-      // The next stage has landed: at most the loads of the one after it are under way, and at a tile's first two stages the
-      // stores of the tile before, which were sent behind those loads.
-      if (k < 2 && stored) __builtin_amdgcn_s_waitcnt(wait_vm(LOADS + STORES));
-      else __builtin_amdgcn_s_waitcnt(wait_vm(LOADS));
-      meet();
-      load_stage();                                            // into the buffer that the stage before was read from
-      const uint32_t next = (buf + 1) & (TBUF - 1);
+    load_from();
+    const uint32_t next = buf ^ 1u, snext = sbuf == 2 ? 0 : sbuf + 1;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-#pragma unroll
-        for (int i = 0; i < MG; ++i) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) mx_mma(acc[i][q * 2 + j], fw[q & 1][j], sw[q & 1][j], fx[i], sx[i]);
-          if (q < 3 && i < 2) read_w(buf, q + 1, i);
-          if (q < 3 && MG == 1) read_w(buf, q + 1, 1);
-          if (q == 3) {
-            if (i < 2) read_w(next, 0, i);
-            if (MG == 1) read_w(next, 0, 1);
-            read_x(next, i);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
+    for (int q = 0; q < 4; ++q) {
+      if (q == 1 || q == 3) {
+        // What the quarters up to the next barrier read has landed: all but the last LOADS loads (and those stores); and this
+        // wavefront's reads are over.  The branch is inside the statement: around a block's end the compiler moves products.
+        asm volatile("s_cmp_lt_i32 %0, 1\n\ts_cbranch_scc1 .Lmxw%=\n\ts_waitcnt vmcnt(%1) lgkmcnt(0)\n\ts_branch .Lmxd%=\n"
+                     ".Lmxw%=:\n\ts_waitcnt vmcnt(%2) lgkmcnt(0)\n.Lmxd%=:"
+                     ::"s"(behind), "n"(LOADS + STORES), "n"(LOADS) : "scc", "memory");
+        --behind;
+        meet();
       }
-      buf = next;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const int ks = g / MG, i = g % MG;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) mx_mma2(acc[i][q * 2 + j], fw[q & 1][j][ks], sw[q & 1][j], fx[i][ks], sx[i], ks);
+#pragma unroll
+        for (int r = g * 4 / G; r < (g + 1) * 4 / G; ++r) {
+          if (q < 3) read_w(buf, q + 1, r & 1, r >> 1);
+          else read_w(next, 0, r & 1, r >> 1);
+          if (r < 2) { if (q < 3) read_ws(sbuf, q + 1, r); else read_ws(snext, 0, r); }
+        }
+        if (q == 3) {
+          read_x(next, i, ks);
+          if (ks == 1) read_xs(snext, i);
+        }
+        if (q == 1 || q == 2) {
+#pragma unroll
+          for (int r = ((q - 1) * G + g) * FIRST / (2 * G); r < ((q - 1) * G + g + 1) * FIRST / (2 * G); ++r) load_first(r);
+        }
+        if (q == 3 && g < REST) load_rest(g);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
-    // ---- the tile goes out: a lane holds four neighbouring features of token l15 of each group of 16 tokens
+    load_next();
+    buf = next;
+    sbuf = snext;
+    }
+    // ---- the tile goes out: a lane holds four neighbouring features of token l15 of each group of 16 tokens.  They pass
+    // through LDS, so that a store is 16 bytes per lane and 128 neighbouring bytes per token.
     const int n1 = at.n0 + wn * 128;
     const bool whole = at.m0 + BM <= a.M && at.n0 + TN <= a.N;
-    OutT *out = pre + (int64_t)at.layer * a.ps + (int64_t)(at.m0 + wm * 16 * MG) * a.pre_row + n1;
+    // addresses are rebuilt from the lane number for every tile: as loop invariants they would live across the K loop
+    int le = lane;
+    asm volatile("" : "+v"(le));
+    const int c15 = le & 15, cq = le >> 4;
     unsigned char *park = parked + wave * PARK;
-    if (bias) {
-      const OutT *bp = bias + (int64_t)at.layer * a.bs + n1 + lq * 4;
+    constexpr int PE = 16 / (int)sizeof(OutT), JH = HF / 16;
+    OutT *op = pre + (int64_t)at.layer * a.ps + (int64_t)(at.m0 + wm * 16 * MG + (le >> 3)) * a.pre_row + n1 + (le & 7) * PE;
+    if (tile + step < last_tile) load_bias(tile + step);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (at.n0 + TN <= a.N) __builtin_memcpy(bv[j], bp + j * 16, 4 * sizeof(OutT));
-        else
+    for (int h = 0; h < 128 / HF; ++h) {
+      float4 bv[JH];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) bv[j][q] = bp[min(j * 16 + q, a.N - 1 - n1 - lq * 4)];
-      }
-    }
+      for (int jj = 0; jj < JH; ++jj) bv[jj] = *reinterpret_cast<const float4 *>(&bias_lds[wave][h * HF + jj * 16 + cq * 4]);
 #pragma unroll
-    for (int i = 0; i < MG; ++i) {
+      for (int i = 0; i < MG; ++i) {
 #pragma unroll
-      for (int h = 0; h < 128 / HF; ++h) {
-#pragma unroll
-        for (int jj = 0; jj < HF / 16; ++jj) {
-          const int j = h * (HF / 16) + jj;
-          float y[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            y[q] = acc[i][j][q] + (bias ? Elem<OutT>::to_f32(bv[j][q]) : 0.0f);
-            acc[i][j][q] = 0.0f;
-          }
+        for (int jj = 0; jj < JH; ++jj) {
+          const int j = h * JH + jj;
+          const float y[4] = {acc[i][j][0] + bv[jj].x, acc[i][j][1] + bv[jj].y, acc[i][j][2] + bv[jj].z, acc[i][j][3] + bv[jj].w};
+          acc[i][j] = mx_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
           if constexpr (sizeof(OutT) == 4) {
-            const int slot = (jj * 4 + lq) ^ (l15 & 7);
-            *reinterpret_cast<float4 *>(park + l15 * 128 + slot * 16) = make_float4(y[0], y[1], y[2], y[3]);
+            const int slot = (jj * 4 + cq) ^ (c15 & 7);
+            *reinterpret_cast<float4 *>(park + c15 * 128 + slot * 16) = make_float4(y[0], y[1], y[2], y[3]);
           } else {
-            const int slot = (jj * 2 + (lq >> 1)) ^ (l15 & 7);
-            *reinterpret_cast<uint2 *>(park + l15 * 128 + slot * 16 + (lq & 1) * 8) = make_uint2(pack_pair<OutT>(y[0], y[1]), pack_pair<OutT>(y[2], y[3]));
+            const int slot = (jj * 2 + (cq >> 1)) ^ (c15 & 7);
+            *reinterpret_cast<uint2 *>(park + c15 * 128 + slot * 16 + (cq & 1) * 8) = make_uint2(mx_pack<OutT>(y[0], y[1]), mx_pack<OutT>(y[2], y[3]));
           }
         }
+        if (whole) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          constexpr int PE = 16 / (int)sizeof(OutT);
-          const int row = u * 8 + (lane >> 3), sl = lane & 7;
-          const uint4 v = *reinterpret_cast<const uint4 *>(park + row * 128 + ((sl ^ (row & 7)) * 16));
-          OutT *op = out + (int64_t)(i * 16 + row) * a.pre_row + h * HF + sl * PE;
-          if (whole) {
-            __builtin_memcpy(op, &v, 16);
-          } else if (at.m0 + wm * 16 * MG + i * 16 + row < a.M) {
-            const int left = a.N - (n1 + h * HF + sl * PE);
-            if (left >= PE) __builtin_memcpy(op, &v, 16);
-            else {
-              OutT e[PE];
-              __builtin_memcpy(e, &v, 16);
-#pragma unroll
-              for (int q = 0; q < PE; ++q)
-                if (q < left) op[q] = e[q];
-            }
+          for (int u = 0; u < 2; ++u) {
+            const int row = u * 8 + (le >> 3);
+            const uint4 v = *reinterpret_cast<const uint4 *>(park + row * 128 + (((le & 7) ^ (row & 7)) * 16));
+            __builtin_memcpy(op + (int64_t)(i * 16 + u * 8) * a.pre_row + h * HF, &v, 16);
+          }
+        } else {
+#pragma clang loop unroll(disable)
+          for (int u = 0; u < 2; ++u) {
+            const int row = u * 8 + (le >> 3), left = min(a.N - (n1 + h * HF + (le & 7) * PE), PE);
+            const OutT *vp = reinterpret_cast<const OutT *>(park + row * 128 + (((le & 7) ^ (row & 7)) * 16));
+            if (at.m0 + wm * 16 * MG + i * 16 + row < a.M)
+#pragma clang loop unroll(disable)
+              for (int q = 0; q < left; ++q) op[(int64_t)(i * 16 + u * 8) * a.pre_row + h * HF + q] = vp[q];
           }
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
-    stored = whole;
+    keep_bias();
+    behind = whole ? 3 : 0;
     tile += step;
     if (tile >= last_tile) break;
   }
@@ -626,22 +715,24 @@ int mx_read(int dtype, int fmt, const void *codes, const uint8_t *scales, const 
 // Batches that the tile kernel takes, in tokens.
 constexpr int64_t MX_TILE_MIN_TOKENS = 129;
 
-// What the projection keeps for itself: x in codes, rows of whole stages; the scales of W where their rows are not.
+// What the projection keeps for itself: x in codes, rows of whole stages; the scales of W where its rows are no whole number of
+// words.
 struct MxPlan {
-  int64_t blocks, padded;      // blocks of a row, and in whole stages
+  int64_t blocks, padded, wsblocks;   // blocks of a row; of a row of x in whole stages; bytes of a row of W's scales
   bool tiles;
-  size_t xc, xs, ws, bytes;    // offsets in the workspace
+  size_t xc, xs, ws, bytes;           // offsets in the workspace
 };
 MxPlan mx_plan(int64_t T, int64_t d, int64_t F, int64_t L, bool quantised) {
   MxPlan p{};
   p.blocks = clt_ceil_div(d, 32);
   p.tiles = T >= MX_TILE_MIN_TOKENS;
-  p.padded = p.tiles ? (p.blocks + 3) / 4 * 4 : p.blocks;
+  p.padded = p.tiles ? (p.blocks + TBLOCKS - 1) / TBLOCKS * TBLOCKS : p.blocks;
+  p.wsblocks = p.tiles ? (p.blocks + 3) / 4 * 4 : p.blocks;
   const bool own_x = !quantised || p.padded != p.blocks;
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
   p.xs = up(own_x ? (size_t)(L * T * p.padded * 16) : 0);
   p.ws = p.xs + up(own_x ? (size_t)(L * T * p.padded) : 0);
-  p.bytes = p.ws + up(p.padded != p.blocks ? (size_t)(L * F * p.padded) : 0);
+  p.bytes = p.ws + up(p.wsblocks != p.blocks ? (size_t)(L * F * p.wsblocks) : 0);
   return p;
 }
 
@@ -662,8 +753,8 @@ int launch_mx_project(const MxPlan &p, const uint8_t *xc, const uint8_t *xs, con
     if (total > 1073741824LL) return CLT_ERR_RANGE;
     const int grid = mx_grid(total);
     if (grid <= 0) return CLT_ERR_LAUNCH;
-    TileArgs a{xc, xs, wc, wsc, (int)T, (int)F, (int)tm, (int)tn, (int)total, (int)clt_ceil_div(total, 8), (int)(p.padded / 4),
-               (int)p.padded * 16, (int)p.blocks * 16, (int)p.padded, (int)p.blocks, bs, ps, pre_row};
+    TileArgs a{xc, xs, wc, wsc, (int)T, (int)F, (int)tm, (int)tn, (int)total, (int)clt_ceil_div(total, 8), (int)(p.padded / TBLOCKS),
+               (int)p.padded * 16, (int)p.blocks * 16, (int)p.padded, (int)p.wsblocks, bs, ps, pre_row};
     k_mx_project_tiles<OutT, MG><<<grid, TW * 64, 0, s>>>(a, (const OutT *)bias, (OutT *)pre);
     return clt_check_launch();
   }
@@ -776,7 +867,8 @@ extern "C" int clt_mx_encode(const void *x, const uint8_t *x_scales, const void 
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return CLT_ERR_WORKSPACE;
   if (p.bytes > 0 && !clt_aligned16(workspace)) return CLT_ERR_ALIGN;
   // the tile kernel fetches four scales at a time
-  if (p.tiles && p.padded == p.blocks && (((uintptr_t)w_scales | (uintptr_t)x_scales) & 3u) != 0) return CLT_ERR_ALIGN;
+  if (p.tiles && ((p.wsblocks == p.blocks && ((uintptr_t)w_scales & 3u) != 0) || (p.padded == p.blocks && ((uintptr_t)x_scales & 3u) != 0)))
+    return CLT_ERR_ALIGN;
   hipStream_t s = (hipStream_t)stream;
   uint8_t *ws = (uint8_t *)workspace;
   const uint8_t *xc = (const uint8_t *)x, *xs = x_scales, *wc = (const uint8_t *)w_codes, *wsc = w_scales;
@@ -792,8 +884,8 @@ extern "C" int clt_mx_encode(const void *x, const uint8_t *x_scales, const void 
     xc = ws + p.xc;
     xs = ws + p.xs;
   }
-  if (rc == CLT_OK && p.padded != p.blocks) {
-    rc = launch_mx_widen(w_scales, ws + p.ws, L * F, p.blocks, p.padded, 1, s);
+  if (rc == CLT_OK && p.wsblocks != p.blocks) {
+    rc = launch_mx_widen(w_scales, ws + p.ws, L * F, p.blocks, p.wsblocks, 1, s);
     wsc = ws + p.ws;
   }
   if (rc != CLT_OK) return rc;
