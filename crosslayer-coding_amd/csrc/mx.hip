@@ -9,12 +9,23 @@
 //     CLT_MXFP8    sign, four bits of exponent, three of mantissa, up to 448
 //     CLT_MXINT8   two's complement in 64ths, -127/64 .. 127/64
 // A row of d elements has ceil(d / 32) blocks; the last one is filled up with zeros.
+#include <type_traits>
 #include "clt_common.h"
 
 namespace {
 
 constexpr int MX_THREADS = 256;
 constexpr int64_t MX_MAX_WIDTH = 262144;    // elements of a row: the pieces of a workgroup's rows are told apart with 32 bits
+
+// The tiles of the projection: MX_BM tokens (four wavefronts of MX_MG groups of 16) x TN features, K in stages of TBLOCKS blocks.
+constexpr int MX_MG = 4, MX_BM = 64 * MX_MG, TN = 256, TBLOCKS = 8;
+
+// Where the scale of block b of row r of a tile lies among those of its stage.  The rows of a wavefront are `groups` groups of
+// 16; a lane's bytes are neighbours, ordered by group and block.
+__host__ __device__ __forceinline__ uint32_t mx_scale_place(uint32_t r, uint32_t b, uint32_t groups) {
+  const uint32_t w = r / (16 * groups), i = r / 16 % groups, lane = (b & 3) * 16 + (r & 15);
+  return (w * 64 + lane) * groups * 2 + i * 2 + (b >> 2);
+}
 
 template <int FMT> struct Mx;
 template <> struct Mx<CLT_MXFP4> { static constexpr int EMAX = 2, BLOCK_BYTES = 16; };
@@ -106,12 +117,12 @@ __device__ __forceinline__ MxPiece mx_piece(uint32_t pieces, uint32_t magic) {
 }
 
 // grid: x = groups of pieces, y = layer * kinds + kind.  Four lanes hold a block and agree on its scale.  `blocks` of a stored row: those
-// behind d are zeros.
+// behind d are zeros.  tiled: scales as the projection's tiles of MX_BM rows take them.
 template <typename T, int FMT, bool VEC>
 __global__ __launch_bounds__(MX_THREADS) void k_mx_write(const T *__restrict__ src0, const T *__restrict__ src1, int64_t layer_stride,
                                                          int64_t row_stride, int kinds, int64_t n, int64_t d, uint32_t blocks,
                                                          uint32_t magic, MxRows rows, uint8_t *__restrict__ codes,
-                                                         uint8_t *__restrict__ scales) {
+                                                         uint8_t *__restrict__ scales, int tiled) {
   const MxPiece at = mx_piece(blocks * 4u, magic);
   const int64_t l = blockIdx.y / (uint32_t)kinds;
   const int kind = (int)(blockIdx.y - (uint32_t)l * (uint32_t)kinds);
@@ -157,7 +168,11 @@ __global__ __launch_bounds__(MX_THREADS) void k_mx_write(const T *__restrict__ s
   const uint2 code = mx_encode8<FMT>(v);
   if constexpr (FMT == CLT_MXFP4) *reinterpret_cast<uint32_t *>(codes + row * blocks * 16u + at.p * 4u) = code.x;
   else *reinterpret_cast<uint2 *>(codes + row * blocks * 32u + at.p * 8u) = code;
-  if ((at.p & 3u) == 0u) scales[row * blocks + (at.p >> 2)] = (uint8_t)s;
+  if ((at.p & 3u) == 0u) {
+    const uint32_t b = at.p >> 2;
+    if (!tiled) scales[row * blocks + b] = (uint8_t)s;
+    else scales[row / MX_BM * MX_BM * blocks + (b / 8) * (MX_BM * 8) + mx_scale_place((uint32_t)(row % MX_BM), b % 8, MX_MG)] = (uint8_t)s;
+  }
 }
 
 // Which row of the batch a store row keeps when several name it: the last one.  Cleared, then raised.
@@ -247,11 +262,22 @@ __device__ __forceinline__ void mx_mma(mx_f32x4_t &acc, const uint4 &a, uint32_t
   acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc, 4, 4, 0, (int)sa, 0, (int)sb);
 }
 
-// The same with the scale in byte ks of the word.
-__device__ __forceinline__ void mx_mma2(mx_f32x4_t &acc, const uint4 &a, uint32_t sa, const uint4 &b, uint32_t sb, int ks) {
+// The same onto c, with the scales in bytes ka and kb of their words.
+template <int KA, int KB> __device__ __forceinline__ mx_f32x4_t mx_mma_at(const mx_f32x4_t &c, const uint4 &a, uint32_t sa, const uint4 &b, uint32_t sb) {
   const mx_i32x8_t av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0}, bv = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
-  if (ks == 0) acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc, 4, 4, 0, (int)sa, 0, (int)sb);
-  else acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc, 4, 4, 1, (int)sa, 1, (int)sb);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, KA, (int)sa, KB, (int)sb);
+}
+__device__ __forceinline__ mx_f32x4_t mx_mma2(const mx_f32x4_t &c, const uint4 &a, uint32_t sa, int ka, const uint4 &b, uint32_t sb, int kb) {
+  switch (ka * 4 + kb) {                                       // known where this is unrolled; both bytes are of the same block
+    case 0: return mx_mma_at<0, 0>(c, a, sa, b, sb);
+    case 2: return mx_mma_at<0, 2>(c, a, sa, b, sb);
+    case 5: return mx_mma_at<1, 1>(c, a, sa, b, sb);
+    case 7: return mx_mma_at<1, 3>(c, a, sa, b, sb);
+    case 8: return mx_mma_at<2, 0>(c, a, sa, b, sb);
+    case 10: return mx_mma_at<2, 2>(c, a, sa, b, sb);
+    case 13: return mx_mma_at<3, 1>(c, a, sa, b, sb);
+    default: return mx_mma_at<3, 3>(c, a, sa, b, sb);
+  }
 }
 
 // pre[l][m][n] = b[l][n] + sum over k of x[l][m][k] w[l][n][k].  A wavefront takes 16 NF features x 16 MT tokens, its operands
@@ -312,20 +338,32 @@ __global__ __launch_bounds__(256) void k_mx_project(const uint8_t *__restrict__ 
 
 // ---- the projection of a batch ------------------------------------------------------------------------------------
 // Tiles of BM tokens x 256 features, one persistent workgroup of 8 wavefronts (4 along the tokens, 2 along the features) per CU.
-// A stage is 256 elements of K: 128 bytes of codes per row - whole cache lines - and 8 of scales, brought straight into
-// LDS, chunk c of row r at chunk position c ^ ((r >> 1) & 7), so that the 16 rows of a fragment read lie in all banks.  A lane
-// multiplies the blocks 2 lq and 2 lq + 1 of its row (lq = lane / 16): their scales are neighbours and come in one read.
+// A stage is 256 elements of K: 128 bytes of codes per row - whole cache lines - brought straight into LDS, chunk c of row r at
+// chunk position c ^ ((r >> 1) & 7): a fragment read's lanes are served in sixteens that take half their rows from one quarter of
+// the wavefront and half from the next, and these places lie in all banks for the blocks lq and lq + 4 that a lane multiplies (lq =
+// lane / 16; 2 lq and 2 lq + 1 met in pairs, which cost half of LDS's cycles).  Scales come as the lanes take them (mx_scale_place): one word holds those of
+// two row groups and both blocks.
 //
 // A stage is four quarters of 4 MG products: all tokens of the wavefront x 32 of its features.  The x fragments stay in
 // registers for the stage, each being replaced by the next stage's behind its last use; the W fragments of the next quarter are
-// read under this one's products.  Two barriers: at the first, behind quarter 0, x and the first half of W have been read by
-// everybody, so those loads of the stage after next (and its scales, which have three places) are asked for; at the second,
-// behind quarter 2, the rest.  A load has a stage and a half to arrive.  The stages of all of a workgroup's tiles form one
-// sequence: the first stages of the next tile travel during the last ones of this tile, and its stores during the next.
-constexpr int TN = 256;                       // features of a tile
+// read under this one's products.  Two barriers: behind quarter 0 x and the first half of W have been read by everybody, so those
+// loads of the stage after next (and its scales and biases, which have three places) are asked for; behind quarter 2 the rest.  A
+// load has a stage and a half to arrive.
+//
+// The stages of all of a workgroup's tiles form one sequence, and so do the ends of the tiles: a quarter's accumulators are
+// final behind the last stage's quarter and taken anew in the next tile's first one, which begins from the bias, and in between they
+// go out, piece by piece among the products of the last three quarters and the first ones of the next tile.  A piece is 16 tokens x
+// 128 bytes; it passes through LDS, so that a store is 16 bytes per lane and whole lines.  Stores are buffer stores, whose bounds drop
+// the rows behind the last token: no branch parts the stream of products.  Loads and stores share a counter that runs in order,
+// so the waits for loads allow for the stores sent behind them.
+//
+// Measured on 12 x 4096 x 768 x 24576, bf16 out (2.42 GB: 405 - 450 us for a kernel that does nothing but store these tiles):
+// 647 us, without loads 558, without stores 504, without both 427 (of which the products alone would be 281 at the 6.6 PFLOP/s that
+// the power limit leaves them on random operands).  On 16 x 8192 x 2048 x 16384: 2330 us (3780 TFLOP/s); 4 products of 8192^3:
+// 1010 - 1030 us (4340).  What did not help: groups of 4, 16 or 32 feature tiles in the order of the tiles (650 - 660 us).
 constexpr int TW = 8;                         // wavefronts
 constexpr int TROW = 128;                     // bytes of codes per row and stage
-constexpr int TBLOCKS = 8;                    // blocks per row and stage
+constexpr int NONTEMPORAL = 2;                // of a buffer store: the result is larger than the caches (742 -> 625 us, see below)
 constexpr int PARK = 2048;                    // bytes of a wavefront's piece of the output tile on its way out
 
 // vmcnt(n), nothing asked of the other counters
@@ -334,45 +372,54 @@ constexpr int wait_vm(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0F70; }
 __device__ __forceinline__ uint32_t mx_lds(const void *p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
 }
-// 16 or 4 bytes per lane from base + off straight into LDS, lane i at at + 16 i or 4 i.  Not counted by the compiler: the
-// waits are written out.
+// 16 bytes per lane from base + off straight into LDS, lane i at at + 16 i.  Not counted by the compiler: the waits are written
+// out.
 __device__ __forceinline__ void mx_fill16(const void *base, uint32_t off, uint32_t at) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(at) : "memory");
 }
-__device__ __forceinline__ void mx_fill4(const void *base, uint32_t off, uint32_t at) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "{m0}"(at) : "memory");
+// The same by the lanes of `mask` alone (they lie as before).
+__device__ __forceinline__ void mx_fill16_low(const void *base, uint32_t off, uint32_t at, uint64_t mask) {
+  uint64_t all;
+  asm volatile("s_mov_b64 %0, exec\n\ts_mov_b64 exec, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, %0"
+               : "=&s"(all) : "v"(off), "s"(base), "{m0}"(at), "s"(mask) : "memory");
 }
 
 struct TileArgs {
-  const uint8_t *xc, *xs, *wc, *ws;           // x rows, codes and scales, hold whole stages (zeros behind the end)
-  int M, N, tiles_m, tiles_n, total, per_xcd;
-  int stages, xpitch, wpitch, xspitch, wspitch;   // bytes of a row of codes, of scales
-  int64_t bs, ps, pre_row;
+  const uint8_t *xc, *wc;                     // x rows hold whole stages (zeros behind the end)
+  const uint8_t *xs, *ws;                     // [L][tiles][stages][8 rows of a tile], as the lanes take them (mx_scale_place)
+  const float *bias;                          // [L][tiles_n][256], as the tiles take them
+  int M, xrows, N, tiles_m, tiles_n, total, per_xcd;   // xrows: rows of x per layer that may be read, whole tiles
+  int stages, xpitch, wpitch;                 // bytes of a row of codes
+  int64_t ps, pre_row;
 };
 
 template <typename OutT, int MG>
 __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_mx_project_tiles(
-    TileArgs a, const OutT *__restrict__ bias, OutT *__restrict__ pre) {
+    TileArgs a, OutT *__restrict__ pre) {
   constexpr int BM = 64 * MG;                              // tokens of a tile; a wavefront takes 16 MG x 128
-  constexpr int SI = (BM + TN) / 32;                       // loads of the scales of 32 rows
-  constexpr int FIRST = MG + 2 + 2, REST = 2;              // loads of a stage per wavefront: x, first half of W, scales; rest of W
+  constexpr int FIRST = MG + 2 + 1 + 1, REST = 2;          // loads of a stage per wavefront: x, first half of W, scales, bias; rest of W
   constexpr int LOADS = FIRST + REST;
-  constexpr int STAGE = (BM + TN) * TROW, SST = (BM + TN) * TBLOCKS;
-  constexpr int HF = 128 / (int)sizeof(OutT);              // features of a parked piece: rows of 128 bytes
-  constexpr int STORES = MG * (128 / HF) * 2;              // stores of a whole tile, per wavefront
+  constexpr int STAGE = (BM + TN) * TROW, SST = (BM + TN) * TBLOCKS + TN * 4;   // codes; scales and biases
   constexpr int G = 2 * MG;                                // pairs of products per quarter
-  static_assert(LOADS + STORES < 64, "the wait counter holds 63");
+  constexpr int HF = 128 / (int)sizeof(OutT);              // features of a piece
+  constexpr int JH = HF / 16;                              // and in groups of 16
+  constexpr int PIECES = MG * (128 / HF);                  // of a wavefront's tile
+  constexpr int PQ = PIECES / 4;                           // that go out in each of four quarters,
+  constexpr int LQ0 = HF / 32;                             // of which the first is this one of a tile's last stage (its features are final)
+  constexpr int EQ = 2 * PQ;                               // stores in such a quarter
+  static_assert(BM + TN == TW * 64 && LOADS + 6 * EQ < 64, "a wavefront brings the scales of 64 rows; the wait counter holds 63");
   __shared__ __attribute__((aligned(16))) unsigned char ring[2 * STAGE];
   __shared__ __attribute__((aligned(16))) unsigned char sring[3 * SST];
   __shared__ __attribute__((aligned(16))) unsigned char parked[TW * PARK];
-  __shared__ __attribute__((aligned(16))) float bias_lds[TW][128];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave & 3, wn = wave >> 2, l15 = lane & 15, lq = lane >> 4;
   const uint32_t ring0 = mx_lds(ring), sring0 = mx_lds(sring);
 
   // Block b runs on XCD b % 8 and takes every (gridDim / 8)-th of that XCD's share of the tiles, a run of them in an order
   // that goes through 8 feature tiles for each token tile: the W tiles stay in the XCD's L2 while the tokens pass.
-  struct At { int layer, m0, n0; };
+  // The last feature tile is moved back inside the matrix; what it shares with its neighbour is the same in both.
+  // K is walked from a stage of the tile's own, so that the CUs that share x or W ask for different lines at any one time.
+  struct At { int layer, tm, m0, n0, tn, rot; };
   auto locate = [&](int t) {
     const int per = a.tiles_m * a.tiles_n;
     At at;
@@ -381,8 +428,11 @@ __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const int g = t / (8 * a.tiles_m), r = t - g * 8 * a.tiles_m;
     const int cnt = min(8, a.tiles_n - g * 8);
     const int tm = r / cnt;
+    at.tm = tm;
     at.m0 = tm * BM;
-    at.n0 = (g * 8 + r - tm * cnt) * TN;
+    at.rot = (int)((unsigned)(3 * tm + min(g * 8 + r - tm * cnt, a.tiles_n - 2)) % (unsigned)a.stages);
+    at.tn = g * 8 + r - tm * cnt;
+    at.n0 = min(at.tn * TN, a.N - TN);
     return at;
   };
   const int step = (int)gridDim.x >> 3;
@@ -391,75 +441,67 @@ __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   if (tile >= last_tile) return;
 
   // ---- the loader: where its next stage comes from.  A load of codes brings 8 rows, lane l row l / 8 at chunk position l % 8.
-  int in_tile = tile, in_stage = 0;
-  uint32_t in_buf = 0, in_sbuf = 0, xo[MG], wo[4], so[2];
-  const uint8_t *in_x, *in_w, *in_s[2];
+  int in_tile = tile, in_left = a.stages, in_stage = 0;
+  uint32_t in_buf = 0, in_sbuf = 0;
+  const uint8_t *in_x, *in_w, *in_s;
+  const float *in_b;
   const uint32_t chunkE = (uint32_t)((lane & 7) ^ (lane >> 4)) * 16u;      // groups of 8 rows that begin at 0 mod 16; at 8: ^ 64
   // x: rows 8 MG wave + 8 i.  W: row groups in the order of the quarters, first half 0 .. 63 and 128 .. 191, rest behind them
   auto w_row = [&](int i) { const int u = (i & 1) * 8 + wave; return (i >> 1) * 64 + (u >> 3) * 128 + (u & 7) * 8; };
+  const uint32_t xo = (uint32_t)(lane >> 3) * (uint32_t)a.xpitch + chunkE, wo = (uint32_t)(lane >> 3) * (uint32_t)a.wpitch;
   auto aim = [&]() {
     const At at = locate(in_tile);
-    int la = lane;                                            // rebuilt for every tile, see the epilogue
-    asm volatile("" : "+v"(la));
-    const int lr = la >> 3;
-    in_x = a.xc + ((int64_t)at.layer * a.M + at.m0) * a.xpitch;
+    in_stage = at.rot;
+    in_x = a.xc + ((int64_t)at.layer * a.xrows + at.m0) * a.xpitch;
     in_w = a.wc + ((int64_t)at.layer * a.N + at.n0) * a.wpitch;
-    const int xl = a.M - 1 - at.m0, wl = a.N - 1 - at.n0;     // rows past the end repeat the last one
-#pragma unroll
-    for (int i = 0; i < MG; ++i) {
-      const int r = (wave * MG + i) * 8;
-      xo[i] = (uint32_t)min(r + lr, xl) * (uint32_t)a.xpitch + (chunkE ^ ((r & 8) ? 64u : 0u));
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) wo[i] = (uint32_t)min(w_row(i) + lr, wl) * (uint32_t)a.wpitch;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = (wave * 2 + i) % SI * 32;
-      const bool of_x = r < BM;
-      in_s[i] = of_x ? a.xs + ((int64_t)at.layer * a.M + at.m0) * a.xspitch : a.ws + ((int64_t)at.layer * a.N + at.n0) * a.wspitch;
-      so[i] = (uint32_t)min((of_x ? r : r - BM) + (la >> 1), of_x ? xl : wl) * (uint32_t)(of_x ? a.xspitch : a.wspitch);
-    }
+    // eight wavefronts, 64 rows of scales each: those of x, then those of W
+    in_s = wave * 64 < BM ? a.xs + ((int64_t)at.layer * a.tiles_m + at.tm) * a.stages * (BM * TBLOCKS) + wave * 64 * TBLOCKS
+                          : a.ws + ((int64_t)at.layer * a.tiles_n + at.tn) * a.stages * (TN * TBLOCKS) + (wave * 64 - BM) * TBLOCKS;
+    in_b = a.bias + ((int64_t)at.layer * a.tiles_n + at.tn) * TN;
   };
   // W and its scales are not filled up: behind the end the last block is repeated, and x is zero there
   auto load_w = [&](int i) {
     const int r = w_row(i);
-    mx_fill16(in_w, wo[i] + min((uint32_t)in_stage * TROW + (chunkE ^ ((r & 8) ? 64u : 0u)), (uint32_t)a.wpitch - 16u), ring0 + in_buf * STAGE + (uint32_t)(BM + r) * TROW);
+    mx_fill16(in_w + (uint32_t)r * (uint32_t)a.wpitch, wo + min((uint32_t)in_stage * TROW + (chunkE ^ ((r & 8) ? 64u : 0u)), (uint32_t)a.wpitch - 16u),
+              ring0 + in_buf * STAGE + (uint32_t)(BM + r) * TROW);
   };
   auto load_first = [&](int i) {
-    if (i < MG) mx_fill16(in_x + (int64_t)in_stage * TROW, xo[i], ring0 + in_buf * STAGE + (uint32_t)(wave * MG + i) * (8 * TROW));
-    else if (i < MG + 2) load_w(i - MG);
-    else {
-      const int u = (wave * 2 + i - MG - 2) % SI;
-      const uint32_t pitch = (uint32_t)(u * 32 < BM ? a.xspitch : a.wspitch);
-      mx_fill4(in_s[i - MG - 2], so[i - MG - 2] + min((uint32_t)in_stage * 8u + (uint32_t)(lane & 1) * 4u, pitch - 4u),
-               sring0 + in_sbuf * SST + (uint32_t)u * 256u);
-    }
+    if (i < MG) {
+      const int r = (wave * MG + i) * 8;
+      mx_fill16(in_x + (uint32_t)r * (uint32_t)a.xpitch + (int64_t)in_stage * TROW, xo ^ ((r & 8) ? 64u : 0u), ring0 + in_buf * STAGE + (uint32_t)r * TROW);
+    } else if (i < MG + 2) load_w(i - MG);
+    else if (i == MG + 2)
+      mx_fill16_low(in_s + (int64_t)in_stage * (wave * 64 < BM ? BM * TBLOCKS : TN * TBLOCKS), (uint32_t)lane * 16u,
+                    sring0 + in_sbuf * SST + (uint32_t)(wave * 64 * TBLOCKS), 0xFFFFFFFFull);
+    else
+      mx_fill16_low(in_b + wave * 32, (uint32_t)lane * 16u, sring0 + in_sbuf * SST + (BM + TN) * TBLOCKS + (uint32_t)wave * 128u, 0xFFull);
   };
   auto load_rest = [&](int i) { load_w(2 + i); };
   auto load_next = [&]() {
     in_buf ^= 1u;
     in_sbuf = in_sbuf == 2 ? 0 : in_sbuf + 1;
-    ++in_stage;
+    if (++in_stage == a.stages) in_stage = 0;
+    --in_left;
   };
   auto load_from = [&]() {                                     // in front of a stage's first load
-    if (in_stage != a.stages) return;
-    in_stage = 0;
+    if (in_left != 0) return;
+    in_left = a.stages;
     if (in_tile + step < last_tile) in_tile += step;           // behind the last tile: once more, for nobody
     aim();
   };
 
-  // ---- fragments: row l15 of each group of 16, its blocks 2 lq and 2 lq + 1
+  // ---- fragments: row l15 of each group of 16, its blocks lq and lq + 4
   const uint32_t xat = (uint32_t)(wm * 16 * MG + l15) * TROW, wat = (uint32_t)(BM + wn * 128 + l15) * TROW;
-  const uint32_t xsat = (uint32_t)(wm * 16 * MG + l15) * TBLOCKS + lq * 2, wsat = (uint32_t)(BM + wn * 128 + l15) * TBLOCKS + lq * 2;
-  const uint32_t koff[2] = {(uint32_t)((lq * 2) ^ ((l15 >> 1) & 7)) * 16u, (uint32_t)((lq * 2 + 1) ^ ((l15 >> 1) & 7)) * 16u};
+  const uint32_t xsat = (uint32_t)(wm * 64 + lane) * (MG * 2), wsat = (uint32_t)(BM * TBLOCKS + (wn * 64 + lane) * 16);
+  const uint32_t koff[2] = {(uint32_t)(lq ^ ((l15 >> 1) & 7)) * 16u, (uint32_t)((lq + 4) ^ ((l15 >> 1) & 7)) * 16u};
   uint4 fx[MG][2], fw[2][2][2];
-  uint32_t sx[MG], sw[2][2];
+  uint32_t sx[MG / 2], sw[2];
   auto read_x = [&](uint32_t buf, int i, int ks) { fx[i][ks] = *reinterpret_cast<const uint4 *>(ring + buf * STAGE + xat + i * 16 * TROW + koff[ks]); };
-  auto read_xs = [&](uint32_t sbuf, int i) { sx[i] = *reinterpret_cast<const uint16_t *>(sring + sbuf * SST + xsat + i * 16 * TBLOCKS); };
+  auto read_xs = [&](uint32_t sbuf, int i) { sx[i] = *reinterpret_cast<const uint32_t *>(sring + sbuf * SST + xsat + i * 4); };
   auto read_w = [&](uint32_t buf, int q, int j, int ks) {
     fw[q & 1][j][ks] = *reinterpret_cast<const uint4 *>(ring + buf * STAGE + wat + (q * 2 + j) * 16 * TROW + koff[ks]);
   };
-  auto read_ws = [&](uint32_t sbuf, int q, int j) { sw[q & 1][j] = *reinterpret_cast<const uint16_t *>(sring + sbuf * SST + wsat + (q * 2 + j) * 16 * TBLOCKS); };
+  auto read_ws = [&](uint32_t sbuf, int q) { sw[q & 1] = *reinterpret_cast<const uint32_t *>(sring + sbuf * SST + wsat + q * 4); };
   auto meet = [&]() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -468,29 +510,46 @@ __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     asm volatile("" ::: "memory");
   };
 
-  mx_f32x4_t acc[MG][8];
+  mx_f32x4_t acc[MG][8], bv[2];
+  auto read_bias = [&](uint32_t sbuf, int q) {
 #pragma unroll
-  for (int i = 0; i < MG; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[i][j] = mx_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-
-  // The bias of a tile, two features per lane: asked for in front of the stores of the tile before, so that its arrival does not
-  // wait for them, and put into LDS behind them.
-  float b0 = 0.0f, b1 = 0.0f;
-  auto load_bias = [&](int t) {
-    if (!bias) return;
-    const At at = locate(t);
-    int la = lane;
-    asm volatile("" : "+v"(la));
-    const OutT *bp = bias + (int64_t)at.layer * a.bs;
-    const int n = at.n0 + wn * 128 + la * 2;
-    b0 = Elem<OutT>::to_f32(bp[min(n, a.N - 1)]);
-    b1 = Elem<OutT>::to_f32(bp[min(n + 1, a.N - 1)]);
+    for (int j = 0; j < 2; ++j)
+      bv[j] = *reinterpret_cast<const mx_f32x4_t *>(sring + sbuf * SST + (BM + TN) * TBLOCKS + (wn * 128 + (q * 2 + j) * 16 + lq * 4) * 4);
   };
-  auto keep_bias = [&]() { *reinterpret_cast<float2 *>(&bias_lds[wave][lane * 2]) = make_float2(b0, b1); };
 
-  load_bias(tile);
-  keep_bias();
+  // ---- the way out.  A lane holds four neighbouring features of token l15 of each group of 16 tokens.
+  unsigned char *park = parked + wave * PARK;
+  const uint32_t out_pitch = (uint32_t)a.pre_row * (uint32_t)sizeof(OutT);
+  // Addresses are rebuilt from the lane number by every stage that needs them: as invariants they would live across all others.
+  int la_out = lane;
+  __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(pre, 0, 0, 0x00020000);      // no tile yet: nothing is in bounds
+  auto aim_out = [&](const At &at) {
+    const int rows = min(BM, a.M - at.m0);
+    out = __builtin_amdgcn_make_buffer_rsrc(pre + (int64_t)at.layer * a.ps + (int64_t)at.m0 * a.pre_row + at.n0, 0,
+                                            (int)((uint32_t)(rows - 1) * out_pitch + TN * (uint32_t)sizeof(OutT)), 0x00020000);
+  };
+  auto put = [&](int n) {
+    const int i = n % MG, h = n / MG, l15 = la_out & 15, lq = la_out >> 4;
+#pragma unroll
+    for (int jj = 0; jj < JH; ++jj) {
+      const mx_f32x4_t y = acc[i][h * JH + jj];
+      if constexpr (sizeof(OutT) == 4) {
+        *reinterpret_cast<mx_f32x4_t *>(park + l15 * 128 + ((jj * 4 + lq) ^ (l15 & 7)) * 16) = y;
+      } else {
+        const int slot = (jj * 2 + (lq >> 1)) ^ (l15 & 7);
+        *reinterpret_cast<uint2 *>(park + l15 * 128 + slot * 16 + (lq & 1) * 8) = make_uint2(mx_pack<OutT>(y[0], y[1]), mx_pack<OutT>(y[2], y[3]));
+      }
+    }
+  };
+  typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
+  u32x4_t v;
+  auto take = [&](int u) { v = *reinterpret_cast<const u32x4_t *>(park + (u * 8 + (la_out >> 3)) * 128 + (((la_out & 7) ^ (la_out >> 3)) * 16)); };
+  auto send = [&](int n, int u) {
+    const int i = n % MG, h = n / MG;
+    const uint32_t out_at = (uint32_t)(wm * 16 * MG + (la_out >> 3)) * out_pitch + (uint32_t)(wn * 128 * (int)sizeof(OutT) + (la_out & 7) * 16);
+    __builtin_amdgcn_raw_buffer_store_b128(v, out, (int)(out_at + (uint32_t)(i * 16 + u * 8) * out_pitch + (uint32_t)h * 128u), 0, NONTEMPORAL);
+  };
+
   aim();
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
@@ -504,141 +563,160 @@ __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   __builtin_amdgcn_s_waitcnt(wait_vm(LOADS));                  // the first stage
   meet();
   uint32_t buf = 0, sbuf = 0;
+  read_ws(0, 0);
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    read_ws(0, 0, j);
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) read_w(0, 0, j, ks);
-  }
+  for (int r = 0; r < 4; ++r) read_w(0, 0, r & 1, r >> 1);
+  read_bias(0, 0);
 #pragma unroll
   for (int i = 0; i < MG; ++i) {
-    read_xs(0, i);
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) read_x(0, i, ks);
+    read_x(0, i, 0);
+    read_x(0, i, 1);
+    if (i % 2 == 0) read_xs(0, i / 2);
   }
-  // barriers still to come at which the stores of the tile before are allowed for: STORES of them, no more and no fewer, were
-  // sent behind what these wait for
-  int behind = 0;
 
-  for (;;) {
-    const At at = locate(tile);
-#pragma clang loop unroll(disable)
-    for (int k = 0; k < a.stages; ++k) {
+  // One stage: the first of a tile, the last, both or neither.  At the barriers, what the quarters up to the next barrier read has
+  // landed: all but the last LOADS loads and the stores sent behind what is waited for - in this stage, as its kind says, and
+  // in those before: `late` says that there was a tile before and that this is its first stage, or the second one.  And this
+  // wavefront's reads are over.  (The waits' branch is inside the statement: behind a
+  // block's end the compiler moves products.)
+  auto stage = [&](auto first, auto last, int late, const At &at) {
+    constexpr bool F = decltype(first)::value, E = decltype(last)::value;
+    constexpr int A0 = LOADS + (F ? EQ : 0), A1 = A0 + (F ? (4 - LQ0) * EQ : (LQ0 + 1) * EQ);
+    constexpr int B0 = LOADS + (F ? LQ0 * EQ : 0) + (E ? (3 - LQ0) * EQ : 0), B1 = B0 + (F ? 2 * EQ : 0);
     load_from();
+    if constexpr (F || E) {
+      la_out = lane;
+      asm volatile("" : "+v"(la_out));
+    }
     const uint32_t next = buf ^ 1u, snext = sbuf == 2 ? 0 : sbuf + 1;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      if (q == 1 || q == 3) {
-        // What the quarters up to the next barrier read has landed: all but the last LOADS loads (and those stores); and this
-        // wavefront's reads are over.  The branch is inside the statement: around a block's end the compiler moves products.
-        asm volatile("s_cmp_lt_i32 %0, 1\n\ts_cbranch_scc1 .Lmxw%=\n\ts_waitcnt vmcnt(%1) lgkmcnt(0)\n\ts_branch .Lmxd%=\n"
-                     ".Lmxw%=:\n\ts_waitcnt vmcnt(%2) lgkmcnt(0)\n.Lmxd%=:"
-                     ::"s"(behind), "n"(LOADS + STORES), "n"(LOADS) : "scc", "memory");
-        --behind;
-        meet();
-      }
+      if (q == 1)
+        asm volatile("s_cmp_lg_u32 %0, 0\n\ts_cbranch_scc1 .Lmxl%=\n\ts_waitcnt vmcnt(%1) lgkmcnt(0)\n\ts_branch .Lmxd%=\n"
+                     ".Lmxl%=:\n\ts_waitcnt vmcnt(%2) lgkmcnt(0)\n.Lmxd%=:" ::"s"(late), "n"(A0), "n"(A1) : "scc", "memory");
+      if (q == 3)
+        asm volatile("s_cmp_lg_u32 %0, 0\n\ts_cbranch_scc1 .Lmxl%=\n\ts_waitcnt vmcnt(%1) lgkmcnt(0)\n\ts_branch .Lmxd%=\n"
+                     ".Lmxl%=:\n\ts_waitcnt vmcnt(%2) lgkmcnt(0)\n.Lmxd%=:" ::"s"(late), "n"(B0), "n"(B1) : "scc", "memory");
+      if (q == 1 || q == 3) meet();
+      // the pieces of this quarter: of the tile before in a first stage, of this one in a last
+      const bool out_f = F && q < LQ0, out_e = E && q >= LQ0;
+      if (E && q == LQ0) aim_out(at);
+      const int n0 = out_e ? (q - LQ0) * PQ : (4 - LQ0 + q) * PQ;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const int ks = g / MG, i = g % MG;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) mx_mma2(acc[i][q * 2 + j], fw[q & 1][j][ks], sw[q & 1][j], fx[i][ks], sx[i], ks);
+        for (int j = 0; j < 2; ++j) {
+          mx_f32x4_t &d = acc[i][q * 2 + j];
+          d = mx_mma2(F && ks == 0 ? bv[j] : d, fw[q & 1][j][ks], sw[q & 1], j * 2 + ks, fx[i][ks], sx[i / 2], (i & 1) * 2 + ks);
+        }
 #pragma unroll
         for (int r = g * 4 / G; r < (g + 1) * 4 / G; ++r) {
           if (q < 3) read_w(buf, q + 1, r & 1, r >> 1);
           else read_w(next, 0, r & 1, r >> 1);
-          if (r < 2) { if (q < 3) read_ws(sbuf, q + 1, r); else read_ws(snext, 0, r); }
         }
+        if (g == 0) { if (q < 3) read_ws(sbuf, q + 1); else read_ws(snext, 0); }
+        if (g == MG && ((F && q < 3) || (E && q == 3))) read_bias(q < 3 ? sbuf : snext, (q + 1) & 3);
         if (q == 3) {
           read_x(next, i, ks);
-          if (ks == 1) read_xs(snext, i);
+          if (ks == 1 && i % 2 == 1) read_xs(snext, i / 2);
         }
-        if (q == 1 || q == 2) {
+        // the loads of a quarter lie in front of the stores that the waits count as sent behind them
+        if (q == 1) {
 #pragma unroll
-          for (int r = ((q - 1) * G + g) * FIRST / (2 * G); r < ((q - 1) * G + g + 1) * FIRST / (2 * G); ++r) load_first(r);
+          for (int r = g * FIRST / G; r < (g + 1) * FIRST / G; ++r) load_first(r);
         }
         if (q == 3 && g < REST) load_rest(g);
+        if (out_f || out_e) {
+          constexpr int GP = G / PQ;                           // places of a piece
+          const int e = g / GP, place = g % GP;
+          if (GP >= 4) {
+            if (place == 0) put(n0 + e);
+            if (place == 1) take(0);
+            if (place == 2) { send(n0 + e, 0); take(1); }
+            if (place == 3) send(n0 + e, 1);
+          } else {
+            if (place == 0) { if (e > 0) send(n0 + e - 1, 1); put(n0 + e); take(0); }
+            if (place == 1) { send(n0 + e, 0); take(1); if (e == PQ - 1) send(n0 + e, 1); }
+          }
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    // the products stay in this block: the compiler would move some of them behind its end, next to their next use
+#pragma unroll
+    for (int i = 0; i < MG; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(acc[i][j]));
     load_next();
     buf = next;
     sbuf = snext;
-    }
-    // ---- the tile goes out: a lane holds four neighbouring features of token l15 of each group of 16 tokens.  They pass
-    // through LDS, so that a store is 16 bytes per lane and 128 neighbouring bytes per token.
-    const int n1 = at.n0 + wn * 128;
-    const bool whole = at.m0 + BM <= a.M && at.n0 + TN <= a.N;
-    // addresses are rebuilt from the lane number for every tile: as loop invariants they would live across the K loop
-    int le = lane;
-    asm volatile("" : "+v"(le));
-    const int c15 = le & 15, cq = le >> 4;
-    unsigned char *park = parked + wave * PARK;
-    constexpr int PE = 16 / (int)sizeof(OutT), JH = HF / 16;
-    OutT *op = pre + (int64_t)at.layer * a.ps + (int64_t)(at.m0 + wm * 16 * MG + (le >> 3)) * a.pre_row + n1 + (le & 7) * PE;
-    if (tile + step < last_tile) load_bias(tile + step);
-#pragma unroll
-    for (int h = 0; h < 128 / HF; ++h) {
-      float4 bv[JH];
-#pragma unroll
-      for (int jj = 0; jj < JH; ++jj) bv[jj] = *reinterpret_cast<const float4 *>(&bias_lds[wave][h * HF + jj * 16 + cq * 4]);
-#pragma unroll
-      for (int i = 0; i < MG; ++i) {
-#pragma unroll
-        for (int jj = 0; jj < JH; ++jj) {
-          const int j = h * JH + jj;
-          const float y[4] = {acc[i][j][0] + bv[jj].x, acc[i][j][1] + bv[jj].y, acc[i][j][2] + bv[jj].z, acc[i][j][3] + bv[jj].w};
-          acc[i][j] = mx_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-          if constexpr (sizeof(OutT) == 4) {
-            const int slot = (jj * 4 + cq) ^ (c15 & 7);
-            *reinterpret_cast<float4 *>(park + c15 * 128 + slot * 16) = make_float4(y[0], y[1], y[2], y[3]);
-          } else {
-            const int slot = (jj * 2 + (cq >> 1)) ^ (c15 & 7);
-            *reinterpret_cast<uint2 *>(park + c15 * 128 + slot * 16 + (cq & 1) * 8) = make_uint2(mx_pack<OutT>(y[0], y[1]), mx_pack<OutT>(y[2], y[3]));
-          }
-        }
-        if (whole) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int row = u * 8 + (le >> 3);
-            const uint4 v = *reinterpret_cast<const uint4 *>(park + row * 128 + (((le & 7) ^ (row & 7)) * 16));
-            __builtin_memcpy(op + (int64_t)(i * 16 + u * 8) * a.pre_row + h * HF, &v, 16);
-          }
-        } else {
+  };
+
+  const std::true_type yes;
+  const std::false_type no;
+  int before = 0;
+  for (;;) {
+    const At at = locate(tile);
+    stage(yes, no, before, at);                                // there are at least two
 #pragma clang loop unroll(disable)
-          for (int u = 0; u < 2; ++u) {
-            const int row = u * 8 + (le >> 3), left = min(a.N - (n1 + h * HF + (le & 7) * PE), PE);
-            const OutT *vp = reinterpret_cast<const OutT *>(park + row * 128 + (((le & 7) ^ (row & 7)) * 16));
-            if (at.m0 + wm * 16 * MG + i * 16 + row < a.M)
-#pragma clang loop unroll(disable)
-              for (int q = 0; q < left; ++q) op[(int64_t)(i * 16 + u * 8) * a.pre_row + h * HF + q] = vp[q];
-          }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    keep_bias();
-    behind = whole ? 3 : 0;
+    for (int k = 1; k < a.stages - 1; ++k) stage(no, no, before & (k == 1), at);
+    stage(no, yes, before & (a.stages == 2), at);
+    before = 1;
     tile += step;
     if (tile >= last_tile) break;
+  }
+#pragma unroll
+  for (int n = PIECES - LQ0 * PQ; n < PIECES; ++n) {
+    put(n);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      take(u);
+      send(n, u);
+    }
   }
   __builtin_amdgcn_s_waitcnt(0);   // no load into LDS may be under way when the workgroup ends
 }
 
-// Rows of codes and scales with whole stages of K: the blocks behind the end are zeros.
-__global__ __launch_bounds__(256) void k_mx_widen(const uint8_t *__restrict__ src, uint8_t *__restrict__ dst, int64_t rows, int from, int to,
-                                                  int unit) {
-  const int64_t n = rows * to;
+// What a tile takes beside its codes: the scales of its 256 rows in the lanes' order, zeros where there is no block or no row, and the
+// biases in float32.  grid: x = tiles, y = layers; a thread writes 8 bytes of every stage.
+template <typename T, int GROUPS>
+__global__ __launch_bounds__(256) void k_mx_tile_side(const uint8_t *__restrict__ scales, uint8_t *__restrict__ out, const T *__restrict__ bias,
+                                                      float *__restrict__ bias_out, int rows, int blocks, int stages, int64_t bs) {
+  const int64_t l = blockIdx.y, tile = l * gridDim.x + blockIdx.x;
+  // feature tiles: the last one is moved back inside the matrix
+  const int r0 = GROUPS == 8 ? min((int)blockIdx.x * 256, rows - 256) : (int)blockIdx.x * 256;
+  const int at = threadIdx.x * 8, lane = at / (GROUPS * 2) % 64, w = at / (GROUPS * 128), i0 = at % (GROUPS * 2) / 2;
+  for (int s = 0; s < stages; ++s) {
+    const int b = s * TBLOCKS + (lane >> 4);
+    uint32_t v[2] = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + (w * GROUPS + i0 + i) * 16 + (lane & 15);
+      if (r < rows) {
+        const uint8_t *p = scales + (l * rows + r) * blocks + b;
+        v[i >> 1] |= ((b < blocks ? (uint32_t)p[0] : 0u) | (b + 4 < blocks ? (uint32_t)p[4] << 8 : 0u)) << ((i & 1) * 16);
+      }
+    }
+    *reinterpret_cast<uint2 *>(out + (tile * stages + s) * 2048 + at) = make_uint2(v[0], v[1]);
+  }
+  if (bias_out) bias_out[tile * 256 + threadIdx.x] = bias ? Elem<T>::to_f32(bias[l * bs + r0 + threadIdx.x]) : 0.0f;
+}
+
+// Rows of codes at another pitch, `to` blocks of 16 bytes instead of `from`, filled up with zeros; the rows of a layer `room` rows
+// apart instead of `rows`.
+__global__ __launch_bounds__(256) void k_mx_widen(const uint4 *__restrict__ src, uint4 *__restrict__ dst, int64_t rows, int64_t room, int from, int to) {
+  const int64_t l = blockIdx.y, n = rows * to;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / to;
     const int b = (int)(i - r * to);
-    if (unit == 16) reinterpret_cast<uint4 *>(dst)[i] = b < from ? reinterpret_cast<const uint4 *>(src)[r * from + b] : make_uint4(0u, 0u, 0u, 0u);
-    else dst[i] = b < from ? src[r * from + b] : (uint8_t)0;
+    dst[l * room * to + i] = b < from ? src[(l * rows + r) * from + b] : make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
-int launch_mx_widen(const void *src, void *dst, int64_t rows, int64_t from, int64_t to, int unit, hipStream_t s) {
+int launch_mx_widen(const void *src, void *dst, int64_t L, int64_t rows, int64_t room, int64_t from, int64_t to, hipStream_t s) {
   const int64_t nb = clt_ceil_div(rows * to, 256);
-  k_mx_widen<<<(unsigned)(nb < 65536 ? nb : 65536), 256, 0, s>>>((const uint8_t *)src, (uint8_t *)dst, rows, (int)from, (int)to, unit);
+  k_mx_widen<<<dim3((unsigned)(nb < 65536 ? nb : 65536), (unsigned)L), 256, 0, s>>>((const uint4 *)src, (uint4 *)dst, rows, room, (int)from, (int)to);
   return clt_check_launch();
 }
 
@@ -647,7 +725,7 @@ uint32_t mx_magic(uint32_t pieces) { return (uint32_t)((0x100000000ull + pieces 
 
 template <typename T, int FMT>
 int launch_mx_write(const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t L, int kinds, int64_t n, int64_t d,
-                    uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, hipStream_t s) {
+                    uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, hipStream_t s) {
   const uint32_t pieces = blocks * 4;
   const int64_t groups = clt_ceil_div(n * (int64_t)pieces, MX_THREADS);
   if (groups > 2147483647LL) return CLT_ERR_RANGE;
@@ -656,26 +734,26 @@ int launch_mx_write(const void *src0, const void *src1, int64_t layer_stride, in
   const dim3 grid((unsigned)groups, (unsigned)(L * kinds));
   if (vec)
     k_mx_write<T, FMT, true><<<grid, MX_THREADS, 0, s>>>((const T *)src0, (const T *)src1, layer_stride, row_stride, kinds, n, d, blocks,
-                                                         mx_magic(pieces), rows, (uint8_t *)codes, scales);
+                                                         mx_magic(pieces), rows, (uint8_t *)codes, scales, tiled);
   else
     k_mx_write<T, FMT, false><<<grid, MX_THREADS, 0, s>>>((const T *)src0, (const T *)src1, layer_stride, row_stride, kinds, n, d, blocks,
-                                                          mx_magic(pieces), rows, (uint8_t *)codes, scales);
+                                                          mx_magic(pieces), rows, (uint8_t *)codes, scales, tiled);
   return clt_check_launch();
 }
 
 template <typename T>
 int mx_write_as(int fmt, const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t L, int kinds, int64_t n,
-                int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, hipStream_t s) {
-  if (fmt == CLT_MXFP4) return launch_mx_write<T, CLT_MXFP4>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
-  if (fmt == CLT_MXFP8) return launch_mx_write<T, CLT_MXFP8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
-  return launch_mx_write<T, CLT_MXINT8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
+                int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, hipStream_t s) {
+  if (fmt == CLT_MXFP4) return launch_mx_write<T, CLT_MXFP4>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
+  if (fmt == CLT_MXFP8) return launch_mx_write<T, CLT_MXFP8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
+  return launch_mx_write<T, CLT_MXINT8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
 }
 
 int mx_write(int dtype, int fmt, const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t L, int kinds,
-             int64_t n, int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, hipStream_t s) {
-  if (dtype == CLT_BF16) return mx_write_as<bf16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
-  if (dtype == CLT_F16) return mx_write_as<f16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
-  return mx_write_as<float>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
+             int64_t n, int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, hipStream_t s) {
+  if (dtype == CLT_BF16) return mx_write_as<bf16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
+  if (dtype == CLT_F16) return mx_write_as<f16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
+  return mx_write_as<float>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
 }
 
 template <typename OutT, int FMT>
@@ -712,27 +790,39 @@ int mx_read(int dtype, int fmt, const void *codes, const uint8_t *scales, const 
   return mx_read_as<float>(fmt, codes, scales, rows, L, kinds, n, d, nm, out0, out1, out_layer_stride, out_row_stride, s);
 }
 
-// Batches that the tile kernel takes, in tokens.
+// Batches that the tile kernel takes: at least this many tokens, whole feature tiles, rows of the result at whole words (buffer
+// stores).
 constexpr int64_t MX_TILE_MIN_TOKENS = 129;
+bool mx_tiles_shape(int64_t T, int64_t F) { return T >= MX_TILE_MIN_TOKENS && F >= TN; }
+bool mx_tiles_ok(int64_t T, int64_t F, const void *pre, int64_t ps, int64_t pre_row, int64_t e) {
+  return mx_tiles_shape(T, F) && ((uintptr_t)pre & 3u) == 0 && ps * e % 4 == 0 && pre_row * e % 4 == 0 && F * e % 4 == 0 &&
+         pre_row * e <= (1 << 22);
+}
 
-// What the projection keeps for itself: x in codes, rows of whole stages; the scales of W where its rows are no whole number of
-// words.
+// What the projection keeps for itself: x in codes, in whole tiles of rows of whole stages, its scales and those of W in the lanes'
+// order, the biases of the tiles.  For the other kernels: x in codes as they are.
 struct MxPlan {
-  int64_t blocks, padded, wsblocks;   // blocks of a row; of a row of x in whole stages; bytes of a row of W's scales
-  bool tiles;
-  size_t xc, xs, ws, bytes;           // offsets in the workspace
+  int64_t blocks, padded;             // blocks of a row; of a row of x in whole stages, two at least
+  int64_t xrows, tm, tn, stages;      // rows of x per layer; tiles
+  bool tiles, own_x;
+  size_t xc, xs, ws, bias, bytes;     // offsets in the workspace
 };
-MxPlan mx_plan(int64_t T, int64_t d, int64_t F, int64_t L, bool quantised) {
+MxPlan mx_plan(int64_t T, int64_t d, int64_t F, int64_t L, bool quantised, bool tiles) {
   MxPlan p{};
   p.blocks = clt_ceil_div(d, 32);
-  p.tiles = T >= MX_TILE_MIN_TOKENS;
-  p.padded = p.tiles ? (p.blocks + TBLOCKS - 1) / TBLOCKS * TBLOCKS : p.blocks;
-  p.wsblocks = p.tiles ? (p.blocks + 3) / 4 * 4 : p.blocks;
-  const bool own_x = !quantised || p.padded != p.blocks;
+  p.tiles = tiles;
+  p.padded = tiles ? clt_ceil_div(p.blocks, TBLOCKS) * TBLOCKS : p.blocks;
+  if (tiles && p.padded < 2 * TBLOCKS) p.padded = 2 * TBLOCKS;
+  p.stages = p.padded / TBLOCKS;
+  p.tm = clt_ceil_div(T, MX_BM);
+  p.tn = clt_ceil_div(F, TN);
+  p.xrows = tiles ? p.tm * MX_BM : T;
+  p.own_x = !quantised || p.padded != p.blocks || p.xrows != T;
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
-  p.xs = up(own_x ? (size_t)(L * T * p.padded * 16) : 0);
-  p.ws = p.xs + up(own_x ? (size_t)(L * T * p.padded) : 0);
-  p.bytes = p.ws + up(p.wsblocks != p.blocks ? (size_t)(L * F * p.wsblocks) : 0);
+  p.xs = up(p.own_x ? (size_t)(L * p.xrows * p.padded * 16) : 0);
+  p.ws = p.xs + up(tiles || p.own_x ? (size_t)(L * p.xrows * p.padded) : 0);
+  p.bias = p.ws + (tiles ? (size_t)(L * p.tn * TN * p.padded) : 0);
+  p.bytes = p.bias + (tiles ? (size_t)(L * p.tn * TN * 4) : 0);
   return p;
 }
 
@@ -745,17 +835,18 @@ int mx_grid(int64_t tiles) {
 }
 
 template <typename OutT>
-int launch_mx_project(const MxPlan &p, const uint8_t *xc, const uint8_t *xs, const uint8_t *wc, const uint8_t *wsc, const void *bias, void *pre,
-                      int64_t T, int64_t F, int64_t L, int64_t bs, int64_t ps, int64_t pre_row, hipStream_t s) {
+int launch_mx_project(const MxPlan &p, const uint8_t *xc, const uint8_t *xs, const uint8_t *wc, const uint8_t *wsc, const void *bias,
+                      uint8_t *ws, void *pre, int64_t T, int64_t F, int64_t L, int64_t bs, int64_t ps, int64_t pre_row, hipStream_t s) {
   if (p.tiles) {
-    constexpr int MG = 4;
-    const int64_t tm = clt_ceil_div(T, 64 * MG), tn = clt_ceil_div(F, TN), total = tm * tn * L;
+    const int64_t total = p.tm * p.tn * L;
     if (total > 1073741824LL) return CLT_ERR_RANGE;
     const int grid = mx_grid(total);
     if (grid <= 0) return CLT_ERR_LAUNCH;
-    TileArgs a{xc, xs, wc, wsc, (int)T, (int)F, (int)tm, (int)tn, (int)total, (int)clt_ceil_div(total, 8), (int)(p.padded / TBLOCKS),
-               (int)p.padded * 16, (int)p.blocks * 16, (int)p.padded, (int)p.wsblocks, bs, ps, pre_row};
-    k_mx_project_tiles<OutT, MG><<<grid, TW * 64, 0, s>>>(a, (const OutT *)bias, (OutT *)pre);
+    k_mx_tile_side<OutT, 8><<<dim3((unsigned)p.tn, (unsigned)L), 256, 0, s>>>(wsc, ws + p.ws, (const OutT *)bias, (float *)(ws + p.bias), (int)F,
+                                                                              (int)p.blocks, (int)p.stages, bs);
+    TileArgs a{xc, wc, xs, ws + p.ws, (const float *)(ws + p.bias), (int)T, (int)p.xrows, (int)F, (int)p.tm, (int)p.tn, (int)total,
+               (int)clt_ceil_div(total, 8), (int)p.stages, (int)p.padded * 16, (int)p.blocks * 16, ps, pre_row};
+    k_mx_project_tiles<OutT, MX_MG><<<grid, TW * 64, 0, s>>>(a, (OutT *)pre);
     return clt_check_launch();
   }
   const int blocks = (int)p.blocks;
@@ -793,7 +884,7 @@ extern "C" int clt_mx_quantise(const void *src, int64_t n, int64_t d, int64_t ro
   if (!src || !codes || !scales || (n > 1 && row_stride < d)) return CLT_ERR_ARG;
   if (!clt_aligned16(codes)) return CLT_ERR_ALIGN;
   const MxRows rows{nullptr, 0, 0, n, nullptr};
-  return mx_write(dtype, fmt, src, nullptr, 0, row_stride, 1, 1, n, d, (uint32_t)clt_ceil_div(d, 32), rows, codes, scales, (hipStream_t)stream);
+  return mx_write(dtype, fmt, src, nullptr, 0, row_stride, 1, 1, n, d, (uint32_t)clt_ceil_div(d, 32), rows, codes, scales, 0, (hipStream_t)stream);
 }
 
 extern "C" int clt_mx_dequantise(const void *codes, const uint8_t *scales, int64_t n, int64_t d, int fmt, void *dst, int64_t row_stride,
@@ -826,7 +917,7 @@ extern "C" int clt_mx_cache_write(const void *x, const void *tgt, int64_t layer_
     k_mx_claim<<<nb, 256, 0, s>>>(r, n, owner, 0);
     k_mx_claim<<<nb, 256, 0, s>>>(r, n, owner, 1);
   }
-  return mx_write(dtype, fmt, x, tgt, layer_stride, row_stride, L, 2, n, d, (uint32_t)clt_ceil_div(d, 32), r, codes, scales, s);
+  return mx_write(dtype, fmt, x, tgt, layer_stride, row_stride, L, 2, n, d, (uint32_t)clt_ceil_div(d, 32), r, codes, scales, 0, s);
 }
 
 extern "C" int clt_mx_cache_read(const void *codes, const uint8_t *scales, int64_t rows, int fmt, const void *row_index, int index_bits,
@@ -851,7 +942,9 @@ extern "C" int clt_mx_cache_read(const void *codes, const uint8_t *scales, int64
 
 extern "C" size_t clt_mx_encode_workspace_bytes(int64_t T, int64_t d, int64_t F, int64_t L, int x_quantised) {
   if (T <= 0 || d <= 0 || F <= 0 || L <= 0 || d > MX_MAX_WIDTH) return 0;
-  return mx_plan(T, d, F, L, x_quantised != 0).bytes;
+  const size_t small = mx_plan(T, d, F, L, x_quantised != 0, false).bytes;
+  const size_t tiled = mx_tiles_shape(T, F) ? mx_plan(T, d, F, L, x_quantised != 0, true).bytes : 0;
+  return tiled > small ? tiled : small;
 }
 
 extern "C" int clt_mx_encode(const void *x, const uint8_t *x_scales, const void *w_codes, const uint8_t *w_scales, const void *bias, void *pre,
@@ -863,33 +956,30 @@ extern "C" int clt_mx_encode(const void *x, const uint8_t *x_scales, const void 
   if (!x || !w_codes || !w_scales || !pre || pre_row_stride < F || pre_layer_stride < 0 || (!x_scales && x_layer_stride < 0)) return CLT_ERR_ARG;
   if (d > MX_MAX_WIDTH || T > (1 << 20) || F > (1 << 30) || L > 32767) return CLT_ERR_RANGE;
   if ((x_scales && !clt_aligned16(x)) || !clt_aligned16(w_codes)) return CLT_ERR_ALIGN;
-  const MxPlan p = mx_plan(T, d, F, L, x_scales != nullptr);
-  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return CLT_ERR_WORKSPACE;
-  if (p.bytes > 0 && !clt_aligned16(workspace)) return CLT_ERR_ALIGN;
-  // the tile kernel fetches four scales at a time
-  if (p.tiles && ((p.wsblocks == p.blocks && ((uintptr_t)w_scales & 3u) != 0) || (p.padded == p.blocks && ((uintptr_t)x_scales & 3u) != 0)))
-    return CLT_ERR_ALIGN;
+  const MxPlan p = mx_plan(T, d, F, L, x_scales != nullptr, mx_tiles_ok(T, F, pre, pre_layer_stride, pre_row_stride, clt_elem_bytes(dtype)));
+  const size_t need = clt_mx_encode_workspace_bytes(T, d, F, L, x_scales != nullptr);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return CLT_ERR_WORKSPACE;
+  if (need > 0 && !clt_aligned16(workspace)) return CLT_ERR_ALIGN;
   hipStream_t s = (hipStream_t)stream;
   uint8_t *ws = (uint8_t *)workspace;
-  const uint8_t *xc = (const uint8_t *)x, *xs = x_scales, *wc = (const uint8_t *)w_codes, *wsc = w_scales;
+  const uint8_t *xc = (const uint8_t *)x, *xs = x_scales, *wc = (const uint8_t *)w_codes;
   int rc = CLT_OK;
   if (!x_scales) {
-    const MxRows rows{nullptr, 0, 0, T, nullptr};
-    rc = mx_write(dtype, CLT_MXFP4, x, nullptr, x_layer_stride, d, L, 1, T, d, (uint32_t)p.padded, rows, ws + p.xc, ws + p.xs, s);
+    const MxRows rows{nullptr, 0, 0, p.xrows, nullptr};
+    rc = mx_write(dtype, CLT_MXFP4, x, nullptr, x_layer_stride, d, L, 1, T, d, (uint32_t)p.padded, rows, ws + p.xc, ws + p.xs, p.tiles, s);
     xc = ws + p.xc;
     xs = ws + p.xs;
-  } else if (p.padded != p.blocks) {
-    rc = launch_mx_widen(x, ws + p.xc, L * T, p.blocks, p.padded, 16, s);
-    if (rc == CLT_OK) rc = launch_mx_widen(x_scales, ws + p.xs, L * T, p.blocks, p.padded, 1, s);
-    xc = ws + p.xc;
+  } else if (p.tiles) {
+    if (p.own_x) {
+      rc = launch_mx_widen(x, ws + p.xc, L, T, p.xrows, p.blocks, p.padded, s);
+      xc = ws + p.xc;
+    }
+    k_mx_tile_side<float, MX_MG><<<dim3((unsigned)p.tm, (unsigned)L), 256, 0, s>>>(x_scales, ws + p.xs, nullptr, nullptr, (int)T, (int)p.blocks,
+                                                                                   (int)p.stages, 0);
     xs = ws + p.xs;
-  }
-  if (rc == CLT_OK && p.wsblocks != p.blocks) {
-    rc = launch_mx_widen(w_scales, ws + p.ws, L * F, p.blocks, p.wsblocks, 1, s);
-    wsc = ws + p.ws;
   }
   if (rc != CLT_OK) return rc;
-  if (dtype == CLT_BF16) return launch_mx_project<bf16_t>(p, xc, xs, wc, wsc, bias, pre, T, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s);
-  if (dtype == CLT_F16) return launch_mx_project<f16_t>(p, xc, xs, wc, wsc, bias, pre, T, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s);
-  return launch_mx_project<float>(p, xc, xs, wc, wsc, bias, pre, T, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s);
+  if (dtype == CLT_BF16) return launch_mx_project<bf16_t>(p, xc, xs, wc, w_scales, bias, ws, pre, T, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s);
+  if (dtype == CLT_F16) return launch_mx_project<f16_t>(p, xc, xs, wc, w_scales, bias, ws, pre, T, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s);
+  return launch_mx_project<float>(p, xc, xs, wc, w_scales, bias, ws, pre, T, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s);
 }

@@ -82,8 +82,6 @@ class MXTensor:
                              "do not belong together")
         if codes.data_ptr() % 16 != 0:
             raise ValueError("codes must begin at a multiple of 16 bytes")
-        if scales.data_ptr() % 4 != 0:
-            scales = scales.clone()                 # the kernels fetch four at a time
         self.codes, self.scales, self.fmt, self.width = codes, scales, fmt, int(width)
 
     @property
