@@ -363,7 +363,10 @@ __global__ __launch_bounds__(256) void k_mx_project(const uint8_t *__restrict__ 
 // 1010 - 1030 us (4340).  What did not help: groups of 4, 16 or 32 feature tiles in the order of the tiles (650 - 660 us).
 constexpr int TW = 8;                         // wavefronts
 constexpr int TROW = 128;                     // bytes of codes per row and stage
-constexpr int NONTEMPORAL = 2;                // of a buffer store: the result is larger than the caches (742 -> 625 us, see below)
+// Of a buffer store, taken where the rows of the result begin with a cache line (LINES): its parts are whole lines, and past the caches
+// they go out faster (12 x 4096 x 768 x 24576: 742 -> 625 us).  Elsewhere the L2 has to put lines together (6 x 301 x 640 x 10006,
+// float32: 31 us, and 69 past the caches).
+constexpr int NONTEMPORAL = 2;
 constexpr int PARK = 2048;                    // bytes of a wavefront's piece of the output tile on its way out
 
 // vmcnt(n), nothing asked of the other counters
@@ -393,7 +396,7 @@ struct TileArgs {
   int64_t ps, pre_row;
 };
 
-template <typename OutT, int MG>
+template <typename OutT, int MG, bool LINES>
 __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_mx_project_tiles(
     TileArgs a, OutT *__restrict__ pre) {
   constexpr int BM = 64 * MG;                              // tokens of a tile; a wavefront takes 16 MG x 128
@@ -547,7 +550,7 @@ __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   auto send = [&](int n, int u) {
     const int i = n % MG, h = n / MG;
     const uint32_t out_at = (uint32_t)(wm * 16 * MG + (la_out >> 3)) * out_pitch + (uint32_t)(wn * 128 * (int)sizeof(OutT) + (la_out & 7) * 16);
-    __builtin_amdgcn_raw_buffer_store_b128(v, out, (int)(out_at + (uint32_t)(i * 16 + u * 8) * out_pitch + (uint32_t)h * 128u), 0, NONTEMPORAL);
+    __builtin_amdgcn_raw_buffer_store_b128(v, out, (int)(out_at + (uint32_t)(i * 16 + u * 8) * out_pitch + (uint32_t)h * 128u), 0, LINES ? NONTEMPORAL : 0);
   };
 
   aim();
@@ -846,7 +849,11 @@ int launch_mx_project(const MxPlan &p, const uint8_t *xc, const uint8_t *xs, con
                                                                               (int)p.blocks, (int)p.stages, bs);
     TileArgs a{xc, wc, xs, ws + p.ws, (const float *)(ws + p.bias), (int)T, (int)p.xrows, (int)F, (int)p.tm, (int)p.tn, (int)total,
                (int)clt_ceil_div(total, 8), (int)p.stages, (int)p.padded * 16, (int)p.blocks * 16, ps, pre_row};
-    k_mx_project_tiles<OutT, MX_MG><<<grid, TW * 64, 0, s>>>(a, (OutT *)pre);
+    const int64_t e = sizeof(OutT);
+    if (((uintptr_t)pre & 127u) == 0 && pre_row * e % 128 == 0 && ps * e % 128 == 0)
+      k_mx_project_tiles<OutT, MX_MG, true><<<grid, TW * 64, 0, s>>>(a, (OutT *)pre);
+    else
+      k_mx_project_tiles<OutT, MX_MG, false><<<grid, TW * 64, 0, s>>>(a, (OutT *)pre);
     return clt_check_launch();
   }
   const int blocks = (int)p.blocks;
