@@ -64,6 +64,7 @@ template <int FMT> __device__ __forceinline__ uint2 mx_encode8(const float (&v)[
 }
 
 typedef __attribute__((ext_vector_type(2))) float mx_f32x2_t;
+typedef __attribute__((ext_vector_type(4))) unsigned int mx_u32x4_t;
 typedef __attribute__((ext_vector_type(2))) __bf16 mx_bf16x2_t;
 typedef __attribute__((ext_vector_type(2))) _Float16 mx_f16x2_t;
 
@@ -105,8 +106,10 @@ __device__ __forceinline__ int64_t mx_row(const MxRows &r, int64_t j) {
   return r.wide ? ((const int64_t *)r.index)[j] : (int64_t)((const int32_t *)r.index)[j];
 }
 
-// A workgroup takes 256 neighbouring pieces of eight elements: row and place in it from 32-bit numbers counted from the
-// group's first row.  magic = ceil(2^32 / pieces), exact for counts up to MX_MAX_WIDTH / 8 + 256.
+// A workgroup takes 256 neighbouring pieces: row and place in it from 32-bit numbers counted from the group's first row.
+// magic = ceil(2^32 / pieces), exact for counts up to MX_MAX_WIDTH / 4 + 256 (their product with `pieces` stays below 2^32).
+// A thread goes on to the same piece of `rows_apart` rows further on, so that several loads are under way and what belongs to
+// the column is fetched once.
 struct MxPiece { int64_t j; uint32_t p; };
 __device__ __forceinline__ MxPiece mx_piece(uint32_t pieces, uint32_t magic) {
   const uint64_t base = (uint64_t)blockIdx.x * MX_THREADS;
@@ -116,67 +119,78 @@ __device__ __forceinline__ MxPiece mx_piece(uint32_t pieces, uint32_t magic) {
   return {(int64_t)(row0 + dj), at - dj * pieces};
 }
 
-// grid: x = groups of pieces, y = layer * kinds + kind.  Four lanes hold a block and agree on its scale.  `blocks` of a stored row: those
-// behind d are zeros.  tiled: scales as the projection's tiles of MX_BM rows take them.
+// Eight elements from sp on (those in front of `left` are there), as floats.
+template <typename T, bool VEC> __device__ __forceinline__ void mx_load8(const T *sp, int64_t left, float *v) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+  if constexpr (VEC) {
+    if (left > 0) {                                    // whole pieces
+      if constexpr (sizeof(T) == 2) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(sp);
+        unpack_pair<T>(w.x, v[0], v[1]); unpack_pair<T>(w.y, v[2], v[3]); unpack_pair<T>(w.z, v[4], v[5]); unpack_pair<T>(w.w, v[6], v[7]);
+      } else {
+        const float4 a = *reinterpret_cast<const float4 *>(sp), b = *reinterpret_cast<const float4 *>(sp + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < left) v[k] = Elem<T>::to_f32(sp[k]);
+  }
+}
+
+// The scale byte of the block that two neighbouring lanes hold a half of each; v is scaled for it.
+template <int FMT> __device__ __forceinline__ uint32_t mx_scale16(float (&v)[16]) {
+  uint32_t top = 0;                                    // magnitudes in the order of their bits: NaN above infinity above all numbers
+#pragma unroll
+  for (int k = 0; k < 16; ++k) top = max(top, __float_as_uint(v[k]) & 0x7FFFFFFFu);
+  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xf, 0xf, false));   // quad_perm [1,0,3,2]
+  const uint32_t expo = top >> 23;
+  const uint32_t s = expo <= (uint32_t)Mx<FMT>::EMAX ? 0u : expo - (uint32_t)Mx<FMT>::EMAX;
+  const float up = expo == 255u ? 0.0f : mx_power(254u - s);
+#pragma unroll
+  for (int k = 0; k < 16; ++k) v[k] = expo == 255u ? 0.0f : v[k] * up;
+  return expo == 255u ? 255u : s;
+}
+
+// grid: x = groups of pieces, y = layer * kinds + kind.  A piece is half a block: two lanes agree on its scale.  `blocks` of a stored
+// row: those behind d are zeros.  tiled: scales as the projection's tiles of MX_BM rows take them.
+//
+// Bound by memory: 12 x 24576 rows of 768 bf16 to mxfp4 106 us (573 MB, 5.4 TB/s; past the caches 140 us); 12 layers of 4096 x 768 bf16,
+// inputs and targets, into mxfp8 49 us from memory, 28 us where the batch is still in the memory-side cache.
 template <typename T, int FMT, bool VEC>
 __global__ __launch_bounds__(MX_THREADS) void k_mx_write(const T *__restrict__ src0, const T *__restrict__ src1, int64_t layer_stride,
                                                          int64_t row_stride, int kinds, int64_t n, int64_t d, uint32_t blocks,
                                                          uint32_t magic, MxRows rows, uint8_t *__restrict__ codes,
                                                          uint8_t *__restrict__ scales, int tiled) {
-  const MxPiece at = mx_piece(blocks * 4u, magic);
+  const MxPiece at = mx_piece(blocks * 2u, magic);
+  if (at.j >= n) return;                               // whole pairs: a row has whole blocks
   const int64_t l = blockIdx.y / (uint32_t)kinds;
   const int kind = (int)(blockIdx.y - (uint32_t)l * (uint32_t)kinds);
-  const int64_t c = (int64_t)at.p * 8;
-  const bool live = at.j < n;
-  float v[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-  if (live) {
-    const T *sp = (kind ? src1 : src0) + l * layer_stride + at.j * row_stride + c;
-    if constexpr (VEC) {
-      if (c < d) {                                     // d is a multiple of 8
-        if constexpr (sizeof(T) == 2) {
-          const uint4 w = *reinterpret_cast<const uint4 *>(sp);
-          unpack_pair<T>(w.x, v[0], v[1]); unpack_pair<T>(w.y, v[2], v[3]); unpack_pair<T>(w.z, v[4], v[5]); unpack_pair<T>(w.w, v[6], v[7]);
-        } else {
-          const float4 a = *reinterpret_cast<const float4 *>(sp), b = *reinterpret_cast<const float4 *>(sp + 4);
-          v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (c + k < d) v[k] = Elem<T>::to_f32(sp[k]);
-    }
-  }
-  uint32_t top = 0;                                    // magnitudes in the order of their bits: NaN above infinity above all numbers
-#pragma unroll
-  for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7FFFFFFFu);
-  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xf, 0xf, false));   // quad_perm [1,0,3,2]
-  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xf, 0xf, false));   // quad_perm [2,3,0,1]
-  const uint32_t expo = top >> 23;
-  uint32_t s = expo <= (uint32_t)Mx<FMT>::EMAX ? 0u : expo - (uint32_t)Mx<FMT>::EMAX;
-  const float up = expo == 255u ? 0.0f : mx_power(254u - s);
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = expo == 255u ? 0.0f : v[k] * up;
-  if (expo == 255u) s = 255u;
-  if (!live) return;
+  const int64_t c = (int64_t)at.p * 16;
+  const T *sp = (kind ? src1 : src0) + l * layer_stride + at.j * row_stride + c;
+  float v[16];
+  mx_load8<T, VEC>(sp, d - c, v);
+  mx_load8<T, VEC>(sp + 8, d - c - 8, v + 8);
   const int64_t r = mx_row(rows, at.j);
+  const uint32_t s = mx_scale16<FMT>(v);
   if (r < 0 || r >= rows.rows) return;                 // a row outside the store is not written
   if (rows.owner && rows.owner[r] != (int32_t)at.j) return;
   const uint64_t row = ((uint64_t)l * (uint32_t)kinds + (uint32_t)kind) * (uint64_t)rows.rows + (uint64_t)r;
-  const uint2 code = mx_encode8<FMT>(v);
-  if constexpr (FMT == CLT_MXFP4) *reinterpret_cast<uint32_t *>(codes + row * blocks * 16u + at.p * 4u) = code.x;
-  else *reinterpret_cast<uint2 *>(codes + row * blocks * 32u + at.p * 8u) = code;
-  if ((at.p & 3u) == 0u) {
-    const uint32_t b = at.p >> 2;
-    if (!tiled) scales[row * blocks + b] = (uint8_t)s;
-    else scales[row / MX_BM * MX_BM * blocks + (b / 8) * (MX_BM * 8) + mx_scale_place((uint32_t)(row % MX_BM), b % 8, MX_MG)] = (uint8_t)s;
+  const uint2 a = mx_encode8<FMT>(*reinterpret_cast<float (*)[8]>(v)), b = mx_encode8<FMT>(*reinterpret_cast<float (*)[8]>(v + 8));
+  if constexpr (FMT == CLT_MXFP4) *reinterpret_cast<uint2 *>(codes + row * blocks * 16u + at.p * 8u) = make_uint2(a.x, b.x);
+  else *reinterpret_cast<uint4 *>(codes + row * blocks * 32u + at.p * 16u) = make_uint4(a.x, a.y, b.x, b.y);
+  if ((at.p & 1u) == 0u) {
+    const uint32_t blk = at.p >> 1;
+    if (!tiled) scales[row * blocks + blk] = (uint8_t)s;
+    else scales[row / MX_BM * MX_BM * blocks + (blk / 8) * (MX_BM * 8) + mx_scale_place((uint32_t)(row % MX_BM), blk % 8, MX_MG)] = (uint8_t)s;
   }
 }
 
-// Which row of the batch a store row keeps when several name it: the last one.  Cleared, then raised.
-__global__ void k_mx_claim(MxRows rows, int64_t n, int32_t *owner, int raise) {
+// Which row of the batch a store row keeps when several name it: the last one.  Cleared, then raised: two launches of 1.8 us (one
+// workgroup that does both takes 6.6 us for 501 rows, from one round trip to memory to the next).
+__global__ __launch_bounds__(256) void k_mx_claim(MxRows rows, int64_t n, int32_t *owner, int raise) {
   const int64_t j = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (j >= n) return;
   const int64_t r = mx_row(rows, j);
@@ -191,63 +205,102 @@ struct MxNorm {
   float scale;
 };
 
-template <typename OutT, int FMT, bool VEC>
+// a / s by the reciprocal r of s, corrected once: the quotient rounded to nearest where nothing of it leaves the range of normal
+// numbers.  Eight divisions a thread in the hardware's steps took longer than the bytes (12 layers of 4096 x 768 rows drawn from
+// mxfp8, normalised, to bf16: 67 us, and 49 like this).
+__device__ __forceinline__ float mx_quotient(float a, float s, float r) {
+  const float q = a * r, better = fmaf(fmaf(-q, s, a), r, q);
+  return fabsf(q) <= 0x1p126f ? better : q;
+}
+
+// A thread gives out 16 bytes of U rows: E elements from one place on.  LINES: rows of the result are whole cache lines, so that
+// a wavefront's stores are too; they go past the caches, which would hold back the reads behind them.  12 x 24576 rows of 768 from
+// mxfp4 to bf16: 80 us, and 106 through the caches; 16 layers of 3001 x 2048 rows drawn from mxfp4 to float32, inputs and targets: 124
+// and 231 us.  Two rows a thread: four take 131 us on the second of these.
+template <typename OutT, int FMT, bool VEC, int U, bool LINES>
 __global__ __launch_bounds__(MX_THREADS) void k_mx_read(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, MxRows rows,
-                                                        int64_t n, int64_t d, uint32_t blocks, uint32_t pieces, uint32_t magic, int kinds,
-                                                        MxNorm nm, OutT *__restrict__ out0, OutT *__restrict__ out1,
-                                                        int64_t out_layer_stride, int64_t out_row_stride) {
+                                                        int64_t n, int64_t rows_apart, int64_t d, uint32_t blocks, uint32_t pieces,
+                                                        uint32_t magic, int kinds, MxNorm nm, OutT *__restrict__ out0,
+                                                        OutT *__restrict__ out1, int64_t out_layer_stride, int64_t out_row_stride) {
+  constexpr int E = VEC && sizeof(OutT) == 4 ? 4 : 8;
   const MxPiece at = mx_piece(pieces, magic);
-  if (at.j >= n) return;
+  if (at.j >= rows_apart) return;
   const int64_t l = blockIdx.y / (uint32_t)kinds;
   const int kind = (int)(blockIdx.y - (uint32_t)l * (uint32_t)kinds);
-  const int64_t c = (int64_t)at.p * 8;
-  const int64_t r = mx_row(rows, at.j);
-  float v[8];
-  if (r >= 0 && r < rows.rows) {
-    const uint64_t row = ((uint64_t)l * (uint32_t)kinds + (uint32_t)kind) * (uint64_t)rows.rows + (uint64_t)r;
-    uint2 code = make_uint2(0u, 0u);
-    if constexpr (FMT == CLT_MXFP4) code.x = *reinterpret_cast<const uint32_t *>(codes + row * blocks * 16u + at.p * 4u);
-    else code = *reinterpret_cast<const uint2 *>(codes + row * blocks * 32u + at.p * 8u);
-    const float s = mx_power(scales[row * blocks + (at.p >> 2)]);
-    mx_decode8<FMT>(code, v);
+  const int64_t c = (int64_t)at.p * E;
+  const uint64_t slab = ((uint64_t)l * (uint32_t)kinds + (uint32_t)kind) * (uint64_t)rows.rows;
+  uint2 code[U];
+  uint32_t sb[U];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] *= s;
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(0x7FC00000u);      // a row outside the store is not read
+  for (int u = 0; u < U; ++u) {
+    const int64_t j = at.j + u * rows_apart;
+    const int64_t r = j < n ? mx_row(rows, j) : -1;
+    code[u] = make_uint2(0u, 0u);
+    sb[u] = 255u;                                      // a row outside the store is not read
+    if (r >= 0 && r < rows.rows) {
+      const uint64_t row = slab + (uint64_t)r;
+      const uint8_t *cp = codes + row * blocks * (uint32_t)Mx<FMT>::BLOCK_BYTES + (uint64_t)(FMT == CLT_MXFP4 ? c / 2 : c);
+      if constexpr (FMT == CLT_MXFP4 && E == 4) code[u].x = *reinterpret_cast<const uint16_t *>(cp);
+      else if constexpr (FMT == CLT_MXFP4 || E == 4) code[u].x = *reinterpret_cast<const uint32_t *>(cp);
+      else code[u] = *reinterpret_cast<const uint2 *>(cp);
+      sb[u] = scales[row * blocks + (uint64_t)(c / 32)];
+    }
   }
   const float *mean = kind ? nm.mean1 : nm.mean0, *stdv = kind ? nm.std1 : nm.std0;
-  if (nm.mode == CLT_DENORM_MEAN_STD && mean && stdv) {
-    const float *mp = mean + l * d + c, *tp = stdv + l * d + c;
-    if constexpr (VEC) {
-      const float4 m0 = *reinterpret_cast<const float4 *>(mp), m1 = *reinterpret_cast<const float4 *>(mp + 4);
-      const float4 s0 = *reinterpret_cast<const float4 *>(tp), s1 = *reinterpret_cast<const float4 *>(tp + 4);
-      const float mm[8] = {m0.x, m0.y, m0.z, m0.w, m1.x, m1.y, m1.z, m1.w};
-      const float ss[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = (v[k] - mm[k]) / ss[k];
+  const bool centred = nm.mode == CLT_DENORM_MEAN_STD && mean && stdv;
+  float mm[E], ss[E], rr[E];
+  bool plain = true;                                   // reciprocals that keep the correction among normal numbers
+  if (centred) {
+    if constexpr (VEC) {                               // (of any alignment)
+      __builtin_memcpy(mm, mean + l * d + c, sizeof(mm));
+      __builtin_memcpy(ss, stdv + l * d + c, sizeof(ss));
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (c + k < d) v[k] = (v[k] - mp[k]) / tp[k];
+      for (int k = 0; k < E; ++k) {
+        mm[k] = c + k < d ? mean[l * d + c + k] : 0.0f;
+        ss[k] = c + k < d ? stdv[l * d + c + k] : 1.0f;
+      }
     }
-  } else if (nm.mode == CLT_DENORM_SCALE) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] *= nm.scale;
+    for (int k = 0; k < E; ++k) {
+      const float r = __builtin_amdgcn_rcpf(ss[k]);
+      rr[k] = fmaf(fmaf(-ss[k], r, 1.0f), r, r);
+      plain = plain && fabsf(ss[k]) >= 0x1p-100f && fabsf(ss[k]) <= 0x1p100f;
+    }
   }
-  OutT *op = (kind ? out1 : out0) + l * out_layer_stride + at.j * out_row_stride + c;
-  if constexpr (VEC) {
-    if constexpr (sizeof(OutT) == 2) {
-      *reinterpret_cast<uint4 *>(op) = make_uint4(mx_pack<OutT>(v[0], v[1]), mx_pack<OutT>(v[2], v[3]), mx_pack<OutT>(v[4], v[5]),
-                                                  mx_pack<OutT>(v[6], v[7]));
-    } else {
-      *reinterpret_cast<float4 *>(op) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4 *>(op + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    }
-  } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (c + k < d) op[k] = Elem<OutT>::from_f32(v[k]);
+  for (int u = 0; u < U; ++u) {
+    const int64_t j = at.j + u * rows_apart;
+    if (j >= n) break;
+    float v[8];
+    mx_decode8<FMT>(code[u], v);
+    const float s = mx_power(sb[u]);
+#pragma unroll
+    for (int k = 0; k < E; ++k) v[k] *= s;
+    if (centred) {
+      if (plain) {
+#pragma unroll
+        for (int k = 0; k < E; ++k) v[k] = mx_quotient(v[k] - mm[k], ss[k], rr[k]);
+      } else {
+#pragma clang loop unroll(disable)
+        for (int k = 0; k < E; ++k) v[k] = (v[k] - mean[l * d + min(c + k, d - 1)]) / stdv[l * d + min(c + k, d - 1)];
+      }
+    } else if (nm.mode == CLT_DENORM_SCALE) {
+#pragma unroll
+      for (int k = 0; k < E; ++k) v[k] *= nm.scale;
+    }
+    OutT *op = (kind ? out1 : out0) + l * out_layer_stride + j * out_row_stride + c;
+    if constexpr (!VEC) {
+#pragma unroll
+      for (int k = 0; k < E; ++k)
+        if (c + k < d) op[k] = Elem<OutT>::from_f32(v[k]);
+    } else {
+      mx_u32x4_t o;
+      if constexpr (sizeof(OutT) == 2) o = mx_u32x4_t{mx_pack<OutT>(v[0], v[1]), mx_pack<OutT>(v[2], v[3]), mx_pack<OutT>(v[4], v[5]), mx_pack<OutT>(v[6], v[7])};
+      else o = mx_u32x4_t{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+      if constexpr (LINES) __builtin_nontemporal_store(o, reinterpret_cast<mx_u32x4_t *>(op));
+      else *reinterpret_cast<mx_u32x4_t *>(op) = o;
+    }
   }
 }
 
@@ -724,23 +777,26 @@ int launch_mx_widen(const void *src, void *dst, int64_t L, int64_t rows, int64_t
 }
 
 bool mx_format(int fmt) { return fmt == CLT_MXFP4 || fmt == CLT_MXFP8 || fmt == CLT_MXINT8; }
+// Rows a thread gives out, where that leaves threads enough for the chip: four wavefronts per SIMD.
+constexpr int MX_U = 2;
+constexpr int64_t MX_MANY = 4 * 1024 * 64;
 uint32_t mx_magic(uint32_t pieces) { return (uint32_t)((0x100000000ull + pieces - 1) / pieces); }
 
 template <typename T, int FMT>
 int launch_mx_write(const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t L, int kinds, int64_t n, int64_t d,
                     uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, hipStream_t s) {
-  const uint32_t pieces = blocks * 4;
+  const uint32_t pieces = blocks * 2;
   const int64_t groups = clt_ceil_div(n * (int64_t)pieces, MX_THREADS);
   if (groups > 2147483647LL) return CLT_ERR_RANGE;
   const bool vec = d % 8 == 0 && clt_aligned16(src0) && (kinds == 1 || clt_aligned16(src1)) && (row_stride * (int64_t)sizeof(T)) % 16 == 0 &&
                    (layer_stride * (int64_t)sizeof(T)) % 16 == 0;
   const dim3 grid((unsigned)groups, (unsigned)(L * kinds));
-  if (vec)
-    k_mx_write<T, FMT, true><<<grid, MX_THREADS, 0, s>>>((const T *)src0, (const T *)src1, layer_stride, row_stride, kinds, n, d, blocks,
-                                                         mx_magic(pieces), rows, (uint8_t *)codes, scales, tiled);
-  else
-    k_mx_write<T, FMT, false><<<grid, MX_THREADS, 0, s>>>((const T *)src0, (const T *)src1, layer_stride, row_stride, kinds, n, d, blocks,
-                                                          mx_magic(pieces), rows, (uint8_t *)codes, scales, tiled);
+#define CLT_MXW(VEC)                                                                                                               \
+  k_mx_write<T, FMT, VEC><<<grid, MX_THREADS, 0, s>>>((const T *)src0, (const T *)src1, layer_stride, row_stride, kinds, n, d, blocks, \
+                                                      mx_magic(pieces), rows, (uint8_t *)codes, scales, tiled)
+  if (vec) CLT_MXW(true);
+  else CLT_MXW(false);
+#undef CLT_MXW
   return clt_check_launch();
 }
 
@@ -762,19 +818,24 @@ int mx_write(int dtype, int fmt, const void *src0, const void *src1, int64_t lay
 template <typename OutT, int FMT>
 int launch_mx_read(const void *codes, const uint8_t *scales, const MxRows &rows, int64_t L, int kinds, int64_t n, int64_t d, const MxNorm &nm,
                    void *out0, void *out1, int64_t out_layer_stride, int64_t out_row_stride, hipStream_t s) {
-  const uint32_t blocks = (uint32_t)clt_ceil_div(d, 32), pieces = (uint32_t)clt_ceil_div(d, 8);
-  const int64_t groups = clt_ceil_div(n * (int64_t)pieces, MX_THREADS);
+  constexpr int E = sizeof(OutT) == 4 ? 4 : 8;
+  const int64_t row_bytes = out_row_stride * (int64_t)sizeof(OutT), layer_bytes = out_layer_stride * (int64_t)sizeof(OutT);
+  const bool vec = d % E == 0 && clt_aligned16(out0) && (kinds == 1 || clt_aligned16(out1)) && row_bytes % 16 == 0 && layer_bytes % 16 == 0;
+  const bool lines = d * (int64_t)sizeof(OutT) % 128 == 0 && (((uintptr_t)out0 | (uintptr_t)out1) & 127u) == 0 && row_bytes % 128 == 0 && layer_bytes % 128 == 0;
+  const uint32_t blocks = (uint32_t)clt_ceil_div(d, 32), pieces = (uint32_t)(vec ? d / E : clt_ceil_div(d, 8));
+  const bool many = vec && L * kinds * clt_ceil_div(n, MX_U) * pieces >= MX_MANY;
+  const int64_t apart = many ? clt_ceil_div(n, MX_U) : n, groups = clt_ceil_div(apart * (int64_t)pieces, MX_THREADS);
   if (groups > 2147483647LL) return CLT_ERR_RANGE;
-  const bool vec = d % 8 == 0 && clt_aligned16(out0) && (kinds == 1 || clt_aligned16(out1)) &&
-                   (out_row_stride * (int64_t)sizeof(OutT)) % 16 == 0 && (out_layer_stride * (int64_t)sizeof(OutT)) % 16 == 0 &&
-                   clt_aligned16(nm.mean0) && clt_aligned16(nm.std0) && clt_aligned16(nm.mean1) && clt_aligned16(nm.std1);
   const dim3 grid((unsigned)groups, (unsigned)(L * kinds));
-  if (vec)
-    k_mx_read<OutT, FMT, true><<<grid, MX_THREADS, 0, s>>>((const uint8_t *)codes, scales, rows, n, d, blocks, pieces, mx_magic(pieces), kinds,
-                                                           nm, (OutT *)out0, (OutT *)out1, out_layer_stride, out_row_stride);
-  else
-    k_mx_read<OutT, FMT, false><<<grid, MX_THREADS, 0, s>>>((const uint8_t *)codes, scales, rows, n, d, blocks, pieces, mx_magic(pieces), kinds,
-                                                            nm, (OutT *)out0, (OutT *)out1, out_layer_stride, out_row_stride);
+#define CLT_MXR(VEC, U, LINES)                                                                                                             \
+  k_mx_read<OutT, FMT, VEC, U, LINES><<<grid, MX_THREADS, 0, s>>>((const uint8_t *)codes, scales, rows, n, apart, d, blocks, pieces,           \
+                                                                  mx_magic(pieces), kinds, nm, (OutT *)out0, (OutT *)out1, out_layer_stride, \
+                                                                  out_row_stride)
+  if (many && lines) CLT_MXR(true, MX_U, true);
+  else if (many) CLT_MXR(true, MX_U, false);
+  else if (vec) CLT_MXR(true, 1, false);
+  else CLT_MXR(false, 1, false);
+#undef CLT_MXR
   return clt_check_launch();
 }
 
