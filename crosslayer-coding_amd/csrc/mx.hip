@@ -333,60 +333,151 @@ __device__ __forceinline__ mx_f32x4_t mx_mma2(const mx_f32x4_t &c, const uint4 &
   }
 }
 
-// pre[l][m][n] = b[l][n] + sum over k of x[l][m][k] w[l][n][k].  A wavefront takes 16 NF features x 16 MT tokens, its operands
-// straight from memory; rows past the end repeat the last one and store nothing, blocks past the end count as zeros.
-template <typename OutT, int NF, int MT>
-__global__ __launch_bounds__(256) void k_mx_project(const uint8_t *__restrict__ xc, const uint8_t *__restrict__ xs,
-                                                    const uint8_t *__restrict__ wc, const uint8_t *__restrict__ wsc,
-                                                    const OutT *__restrict__ bias, OutT *__restrict__ pre, int M, int N, int blocks,
-                                                    int64_t bs, int64_t ps, int64_t pre_row) {
+// ---- the projection of few tokens ---------------------------------------------------------------------------------
+// pre[l][m][n] = b[l][n] + sum over k of x[l][m][k] w[l][n][k].  The weights' one pass through the chip is the work: a wavefront
+// takes 32 features x 16 MT tokens, W straight from memory into registers, FEW_STEPS steps of 128 elements of K ahead of the products,
+// also across its features' end; a workgroup goes on to other features of its layer and keeps x, as codes, in LDS.
+// SRC says where x comes from: FEW_VALUES are quantised into LDS by every workgroup, FEW_CODES copied there; FEW_WIDE rows do not
+// fit and are read as they are used.  Rows past the end repeat the last one and store nothing, blocks past the end count as zeros.
+constexpr int FEW_VALUES = 0, FEW_CODES = 1, FEW_WIDE = 2;
+constexpr int FEW_STEPS = 3, FEW_NF = 2, FEW_TN = 4 * 16 * FEW_NF;   // features of a workgroup
+constexpr int FEW_LDS = 80 * 1024;                                   // two workgroups per CU at least
+
+struct FewArgs {
+  const void *x;               // values, or codes
+  const uint8_t *xs, *wc, *ws;
+  int64_t x_layer, bs, ps, pre_row;
+  int M, N, d, blocks, vec;
+};
+__host__ __device__ static inline int few_blocks(int blocks) { return (blocks + 4 * FEW_STEPS - 1) / (4 * FEW_STEPS) * (4 * FEW_STEPS); }
+// a row of codes in LDS: an odd number of 16-byte chunks, so that neighbouring rows begin in other banks
+__host__ __device__ static inline int few_pitch(int blocks) { return few_blocks(blocks) | 1; }
+static inline int few_lds(int blocks, int mt) { return 16 * mt * (few_pitch(blocks) * 16 + few_blocks(blocks)); }
+
+template <typename OutT, int MT, int SRC>
+__global__ __launch_bounds__(256, 2) void k_mx_project_few(FewArgs a, const OutT *__restrict__ bias, OutT *__restrict__ pre) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t few_x[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, lq = lane >> 4;
-  const int64_t layer = blockIdx.z;
-  const int n0 = (blockIdx.x * 4 + wave) * 16 * NF, m0 = blockIdx.y * 16 * MT;
-  if (n0 >= N) return;
-  int64_t wrow[NF], xrow[MT];
+  const int64_t layer = blockIdx.y;
+  const int m0 = blockIdx.z * 16 * MT, P = few_blocks(a.blocks), pitch = few_pitch(a.blocks);
+  uint8_t *few_s = few_x + 16 * MT * pitch * 16;
+  if constexpr (SRC == FEW_VALUES) {
+    const OutT *x = (const OutT *)a.x + layer * a.x_layer;
+    for (int t = threadIdx.x; t < 16 * MT * P * 2; t += 256) {         // half blocks; both halves of one in neighbouring lanes
+      const int r = t / (2 * P), h = t - r * 2 * P, c = h * 16, m = m0 + r;
+      const int left = m < a.M ? a.d - c : 0;
+      const OutT *sp = x + (int64_t)m * a.d + c;
+      float v[16];
+      if (a.vec) {
+        mx_load8<OutT, true>(sp, left, v);
+        mx_load8<OutT, true>(sp + 8, left - 8, v + 8);
+      } else {
+        mx_load8<OutT, false>(sp, left, v);
+        mx_load8<OutT, false>(sp + 8, left - 8, v + 8);
+      }
+      const uint32_t sc = mx_scale16<CLT_MXFP4>(v);
+      const uint2 lo = mx_encode8<CLT_MXFP4>(*reinterpret_cast<float (*)[8]>(v)), hi = mx_encode8<CLT_MXFP4>(*reinterpret_cast<float (*)[8]>(v + 8));
+      *reinterpret_cast<uint2 *>(few_x + (r * pitch + (h >> 1)) * 16 + (h & 1) * 8) = make_uint2(lo.x, hi.x);
+      if ((h & 1) == 0) few_s[r * P + (h >> 1)] = (uint8_t)sc;
+    }
+  }
+  if constexpr (SRC == FEW_CODES) {
+    for (int t = threadIdx.x; t < 16 * MT * P; t += 256) {
+      const int r = t / P, b = t - r * P, m = m0 + r;
+      const bool in = m < a.M && b < a.blocks;
+      const int64_t at = (layer * a.M + (in ? m : 0)) * a.blocks + (in ? b : 0);
+      *reinterpret_cast<uint4 *>(few_x + (r * pitch + b) * 16) = in ? ((const uint4 *)a.x)[at] : make_uint4(0u, 0u, 0u, 0u);
+      few_s[t] = in ? a.xs[at] : (uint8_t)0;
+    }
+  }
+  __syncthreads();
+
+  struct Ahead { uint4 c[FEW_STEPS][FEW_NF]; uint32_t s[FEW_STEPS][FEW_NF]; };
+  const int units = (a.N + FEW_TN - 1) / FEW_TN, chunks = P / (4 * FEW_STEPS);
+  auto fetch = [&](Ahead &f, int unit, int ch) {
 #pragma unroll
-  for (int j = 0; j < NF; ++j) wrow[j] = (layer * N + min(n0 + j * 16 + l15, N - 1)) * blocks;
+    for (int j = 0; j < FEW_NF; ++j) {
+      const int n = min(unit * FEW_TN + (wave * FEW_NF + j) * 16 + l15, a.N - 1);
+      const int64_t row = (layer * a.N + n) * a.blocks;
 #pragma unroll
-  for (int i = 0; i < MT; ++i) xrow[i] = (layer * M + min(m0 + i * 16 + l15, M - 1)) * blocks;
-  mx_f32x4_t acc[MT][NF];
+      for (int t = 0; t < FEW_STEPS; ++t) {
+        const int b = min((ch * FEW_STEPS + t) * 4 + lq, a.blocks - 1);     // behind the end x is zero
+        f.c[t][j] = *reinterpret_cast<const uint4 *>(a.wc + (row + b) * 16);
+        f.s[t][j] = a.ws[row + b];
+      }
+    }
+  };
+  mx_f32x4_t acc[MT][FEW_NF];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < NF; ++j) acc[i][j] = mx_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int kb = 0; kb < blocks; kb += 4) {
-    const bool in = kb + lq < blocks;
-    const int k = in ? kb + lq : blocks - 1;
-    uint4 a[NF], b[MT];
-    uint32_t sa[NF], sb[MT];
+    for (int j = 0; j < FEW_NF; ++j) acc[i][j] = mx_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  auto multiply = [&](const Ahead &f, int ch) {
 #pragma unroll
-    for (int j = 0; j < NF; ++j) { a[j] = *reinterpret_cast<const uint4 *>(wc + (wrow[j] + k) * 16); sa[j] = wsc[wrow[j] + k]; }
+    for (int t = 0; t < FEW_STEPS; ++t) {
+      const int b = (ch * FEW_STEPS + t) * 4 + lq;
 #pragma unroll
-    for (int i = 0; i < MT; ++i) { b[i] = *reinterpret_cast<const uint4 *>(xc + (xrow[i] + k) * 16); sb[i] = xs[xrow[i] + k]; }
-    if (!in) {
+      for (int i = 0; i < MT; ++i) {
+        uint4 xv;
+        uint32_t sv;
+        if constexpr (SRC == FEW_WIDE) {
+          const bool in = b < a.blocks;
+          const int64_t at = (layer * a.M + min(m0 + i * 16 + l15, a.M - 1)) * a.blocks + (in ? b : 0);
+          xv = in ? ((const uint4 *)a.x)[at] : make_uint4(0u, 0u, 0u, 0u);
+          sv = in ? a.xs[at] : 0u;
+        } else {
+          const int r = i * 16 + l15;
+          xv = *reinterpret_cast<const uint4 *>(few_x + (r * pitch + b) * 16);
+          sv = few_s[r * P + b];
+        }
 #pragma unroll
-      for (int j = 0; j < NF; ++j) { a[j] = make_uint4(0u, 0u, 0u, 0u); sa[j] = 0u; }
-#pragma unroll
-      for (int i = 0; i < MT; ++i) { b[i] = make_uint4(0u, 0u, 0u, 0u); sb[i] = 0u; }
-    }
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < NF; ++j) mx_mma(acc[i][j], a[j], sa[j], b[i], sb[i]);
-  }
-  // a lane holds four neighbouring features of token lane % 16
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int m = m0 + i * 16 + l15;
-    if (m >= M) continue;
-#pragma unroll
-    for (int j = 0; j < NF; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int n = n0 + j * 16 + lq * 4 + q;
-        if (n < N) pre[layer * ps + m * pre_row + n] = Elem<OutT>::from_f32(acc[i][j][q] + (bias ? Elem<OutT>::to_f32(bias[layer * bs + n]) : 0.0f));
+        for (int j = 0; j < FEW_NF; ++j) mx_mma(acc[i][j], f.c[t][j], f.s[t][j], xv, sv);
       }
-  }
+    }
+  };
+  // a lane holds four neighbouring features of token lane % 16
+  auto give = [&](int unit) {
+#pragma unroll
+    for (int j = 0; j < FEW_NF; ++j) {
+      const int n = unit * FEW_TN + (wave * FEW_NF + j) * 16 + lq * 4;
+      float bv[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) bv[q] = bias && n < a.N ? Elem<OutT>::to_f32(bias[layer * a.bs + min(n + q, a.N - 1)]) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const int m = m0 + i * 16 + l15;
+        OutT *op = pre + layer * a.ps + m * a.pre_row + n;
+        const float y[4] = {acc[i][j][0] + bv[0], acc[i][j][1] + bv[1], acc[i][j][2] + bv[2], acc[i][j][3] + bv[3]};
+        acc[i][j] = mx_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        if (m >= a.M) continue;
+        if (n + 4 <= a.N) {
+          if constexpr (sizeof(OutT) == 4) __builtin_memcpy(op, y, 16);
+          else {
+            const uint32_t w[2] = {mx_pack<OutT>(y[0], y[1]), mx_pack<OutT>(y[2], y[3])};
+            __builtin_memcpy(op, w, 8);
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (n + q < a.N) op[q] = Elem<OutT>::from_f32(y[q]);
+        }
+      }
+    }
+  };
+  Ahead f0, f1;
+  int unit = blockIdx.x, ch = 0;                        // the grid has no more workgroups per layer than units
+  fetch(f0, unit, 0);
+  auto turn = [&](Ahead &now, Ahead &then) {
+    const bool end = ch + 1 == chunks;
+    const int nunit = end ? unit + (int)gridDim.x : unit, nch = end ? 0 : ch + 1;
+    if (nunit < units) fetch(then, nunit, nch);
+    multiply(now, ch);
+    if (end) give(unit);
+    unit = nunit;
+    ch = nch;
+    return unit < units;
+  };
+  while (turn(f0, f1) && turn(f1, f0)) {}
 }
 
 // ---- the projection of a batch ------------------------------------------------------------------------------------
@@ -854,21 +945,34 @@ int mx_read(int dtype, int fmt, const void *codes, const uint8_t *scales, const 
   return mx_read_as<float>(fmt, codes, scales, rows, L, kinds, n, d, nm, out0, out1, out_layer_stride, out_row_stride, s);
 }
 
-// Batches that the tile kernel takes: at least this many tokens, whole feature tiles, rows of the result at whole words (buffer
-// stores).
-constexpr int64_t MX_TILE_MIN_TOKENS = 129;
-bool mx_tiles_shape(int64_t T, int64_t F) { return T >= MX_TILE_MIN_TOKENS && F >= TN; }
-bool mx_tiles_ok(int64_t T, int64_t F, const void *pre, int64_t ps, int64_t pre_row, int64_t e) {
-  return mx_tiles_shape(T, F) && ((uintptr_t)pre & 3u) == 0 && ps * e % 4 == 0 && pre_row * e % 4 == 0 && F * e % 4 == 0 &&
-         pre_row * e <= (1 << 22);
+// How a shape is computed.  Up to 64 tokens, as long as their rows leave room in LDS for two workgroups per CU, by the kernel for few:
+// W is read once then.  Beyond by tiles, where there are whole feature tiles and rows of the result lie at whole words (buffer
+// stores); else by the kernel for few in groups of tokens.  12 layers, d 768, F 24576, bf16, kernel for few against tiles, us, x
+// quantised in the call: 26 against 46 at 1 token, 30 / 47 at 17, 34 / 47 at 33, 62 / 48 at 77, 78 / 50 at 128, 147 / 59 at 256;
+// 16 layers, d 2048, F 16384: 78 / 100 at 17, 94 / 104 at 64.
+bool mx_tiles_fit(int64_t F, const void *pre, int64_t ps, int64_t pre_row, int64_t e) {
+  return ((uintptr_t)pre & 3u) == 0 && ps * e % 4 == 0 && pre_row * e % 4 == 0 && F * e % 4 == 0 && pre_row * e <= (1 << 22);
 }
+// groups of 16 tokens that the kernel for few takes at a time; 0: not even one fits into LDS
+int mx_few_groups(int64_t T, int64_t blocks) {
+  int mt = T <= 16 ? 1 : T <= 32 ? 2 : T <= 64 ? 4 : 8;
+  while (mt > 0 && (blocks > 65536 || few_lds((int)blocks, mt) > FEW_LDS)) mt >>= 1;
+  return mt;
+}
+bool mx_use_tiles(int64_t T, int64_t F, int64_t blocks) {
+  const int few = mx_few_groups(T, blocks);
+  return F >= TN && T > 16 * (few < 4 ? few : 4);
+}
+
+constexpr int64_t MX_FEW_VALUES = 16384;   // elements of x that every workgroup quantises for itself
 
 // What the projection keeps for itself: x in codes, in whole tiles of rows of whole stages, its scales and those of W in the lanes'
 // order, the biases of the tiles.  For the other kernels: x in codes as they are.
 struct MxPlan {
   int64_t blocks, padded;             // blocks of a row; of a row of x in whole stages, two at least
   int64_t xrows, tm, tn, stages;      // rows of x per layer; tiles
-  bool tiles, own_x;
+  bool tiles, own_x, values;
+  int few;                            // groups of 16 tokens of the kernel for few
   size_t xc, xs, ws, bias, bytes;     // offsets in the workspace
 };
 MxPlan mx_plan(int64_t T, int64_t d, int64_t F, int64_t L, bool quantised, bool tiles) {
@@ -881,7 +985,10 @@ MxPlan mx_plan(int64_t T, int64_t d, int64_t F, int64_t L, bool quantised, bool 
   p.tm = clt_ceil_div(T, MX_BM);
   p.tn = clt_ceil_div(F, TN);
   p.xrows = tiles ? p.tm * MX_BM : T;
-  p.own_x = !quantised || p.padded != p.blocks || p.xrows != T;
+  // few tokens are quantised on the way into LDS, where they fit and a workgroup has not long to go at them
+  p.few = tiles ? 0 : mx_few_groups(T, p.blocks);
+  p.values = !tiles && !quantised && p.few > 0 && 16 * p.few * p.blocks * 32 <= MX_FEW_VALUES;
+  p.own_x = tiles ? !quantised || p.padded != p.blocks || p.xrows != T : !quantised && !p.values;
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
   p.xs = up(p.own_x ? (size_t)(L * p.xrows * p.padded * 16) : 0);
   p.ws = p.xs + up(tiles || p.own_x ? (size_t)(L * p.xrows * p.padded) : 0);
@@ -899,8 +1006,8 @@ int mx_grid(int64_t tiles) {
 }
 
 template <typename OutT>
-int launch_mx_project(const MxPlan &p, const uint8_t *xc, const uint8_t *xs, const uint8_t *wc, const uint8_t *wsc, const void *bias,
-                      uint8_t *ws, void *pre, int64_t T, int64_t F, int64_t L, int64_t bs, int64_t ps, int64_t pre_row, hipStream_t s) {
+int launch_mx_project(const MxPlan &p, const void *xc, int64_t x_layer, bool vec, const uint8_t *xs, const uint8_t *wc, const uint8_t *wsc, const void *bias,
+                      uint8_t *ws, void *pre, int64_t T, int64_t d, int64_t F, int64_t L, int64_t bs, int64_t ps, int64_t pre_row, hipStream_t s) {
   if (p.tiles) {
     const int64_t total = p.tm * p.tn * L;
     if (total > 1073741824LL) return CLT_ERR_RANGE;
@@ -908,7 +1015,7 @@ int launch_mx_project(const MxPlan &p, const uint8_t *xc, const uint8_t *xs, con
     if (grid <= 0) return CLT_ERR_LAUNCH;
     k_mx_tile_side<OutT, 8><<<dim3((unsigned)p.tn, (unsigned)L), 256, 0, s>>>(wsc, ws + p.ws, (const OutT *)bias, (float *)(ws + p.bias), (int)F,
                                                                               (int)p.blocks, (int)p.stages, bs);
-    TileArgs a{xc, wc, xs, ws + p.ws, (const float *)(ws + p.bias), (int)T, (int)p.xrows, (int)F, (int)p.tm, (int)p.tn, (int)total,
+    TileArgs a{(const uint8_t *)xc, wc, xs, ws + p.ws, (const float *)(ws + p.bias), (int)T, (int)p.xrows, (int)F, (int)p.tm, (int)p.tn, (int)total,
                (int)clt_ceil_div(total, 8), (int)p.stages, (int)p.padded * 16, (int)p.blocks * 16, ps, pre_row};
     const int64_t e = sizeof(OutT);
     if (((uintptr_t)pre & 127u) == 0 && pre_row * e % 128 == 0 && ps * e % 128 == 0)
@@ -917,15 +1024,27 @@ int launch_mx_project(const MxPlan &p, const uint8_t *xc, const uint8_t *xs, con
       k_mx_project_tiles<OutT, MX_MG, false><<<grid, TW * 64, 0, s>>>(a, (OutT *)pre);
     return clt_check_launch();
   }
-  const int blocks = (int)p.blocks;
-#define CLT_MXP(NF, MT)                                                                                                          \
-  {                                                                                                                              \
-    const dim3 grid((unsigned)clt_ceil_div(F, 64 * NF), (unsigned)clt_ceil_div(T, 16 * MT), (unsigned)L);                          \
-    k_mx_project<OutT, NF, MT><<<grid, 256, 0, s>>>(xc, xs, wc, wsc, (const OutT *)bias, (OutT *)pre, (int)T, (int)F, blocks, bs, ps, pre_row); \
+  const int mt = p.few > 0 ? p.few : 4, lds = p.few > 0 ? few_lds((int)p.blocks, mt) : 0;
+  const int64_t units = clt_ceil_div(F, FEW_TN), gz = clt_ceil_div(T, 16 * mt);
+  if (gz > 65535) return CLT_ERR_RANGE;
+  // three workgroups per CU where they fit, so that the last ones are not long alone
+  const int64_t room = clt_ceil_div(256 * (lds > 52 * 1024 ? 2 : 3), L * gz), gx = units < room ? units : room;
+  const FewArgs a{xc, xs, wc, wsc, x_layer, bs, ps, pre_row, (int)T, (int)F, (int)d, (int)p.blocks, vec ? 1 : 0};
+  const dim3 grid((unsigned)gx, (unsigned)L, (unsigned)gz);
+#define CLT_FEW(MT, SRC)                                                                                                            \
+  {                                                                                                                                \
+    if (lds > 64 * 1024 && hipFuncSetAttribute((const void *)k_mx_project_few<OutT, MT, SRC>, hipFuncAttributeMaxDynamicSharedMemorySize, \
+                                               lds) != hipSuccess)                                                                 \
+      return CLT_ERR_LAUNCH;                                                                                                       \
+    k_mx_project_few<OutT, MT, SRC><<<grid, 256, lds, s>>>(a, (const OutT *)bias, (OutT *)pre);                                     \
   }
-  if (T <= 16) CLT_MXP(2, 1)
-  else CLT_MXP(4, 4)
-#undef CLT_MXP
+  if (p.few == 0) CLT_FEW(4, FEW_WIDE)
+  else if (p.values) {
+    if (mt == 1) CLT_FEW(1, FEW_VALUES) else if (mt == 2) CLT_FEW(2, FEW_VALUES) else if (mt == 4) CLT_FEW(4, FEW_VALUES) else CLT_FEW(8, FEW_VALUES)
+  } else {
+    if (mt == 1) CLT_FEW(1, FEW_CODES) else if (mt == 2) CLT_FEW(2, FEW_CODES) else if (mt == 4) CLT_FEW(4, FEW_CODES) else CLT_FEW(8, FEW_CODES)
+  }
+#undef CLT_FEW
   return clt_check_launch();
 }
 
@@ -1010,8 +1129,9 @@ extern "C" int clt_mx_cache_read(const void *codes, const uint8_t *scales, int64
 
 extern "C" size_t clt_mx_encode_workspace_bytes(int64_t T, int64_t d, int64_t F, int64_t L, int x_quantised) {
   if (T <= 0 || d <= 0 || F <= 0 || L <= 0 || d > MX_MAX_WIDTH) return 0;
+  // enough for any address and pitch of the result
   const size_t small = mx_plan(T, d, F, L, x_quantised != 0, false).bytes;
-  const size_t tiled = mx_tiles_shape(T, F) ? mx_plan(T, d, F, L, x_quantised != 0, true).bytes : 0;
+  const size_t tiled = mx_use_tiles(T, F, clt_ceil_div(d, 32)) ? mx_plan(T, d, F, L, x_quantised != 0, true).bytes : 0;
   return tiled > small ? tiled : small;
 }
 
@@ -1024,15 +1144,19 @@ extern "C" int clt_mx_encode(const void *x, const uint8_t *x_scales, const void 
   if (!x || !w_codes || !w_scales || !pre || pre_row_stride < F || pre_layer_stride < 0 || (!x_scales && x_layer_stride < 0)) return CLT_ERR_ARG;
   if (d > MX_MAX_WIDTH || T > (1 << 20) || F > (1 << 30) || L > 32767) return CLT_ERR_RANGE;
   if ((x_scales && !clt_aligned16(x)) || !clt_aligned16(w_codes)) return CLT_ERR_ALIGN;
-  const MxPlan p = mx_plan(T, d, F, L, x_scales != nullptr, mx_tiles_ok(T, F, pre, pre_layer_stride, pre_row_stride, clt_elem_bytes(dtype)));
+  const int64_t e = clt_elem_bytes(dtype);
+  const MxPlan p = mx_plan(T, d, F, L, x_scales != nullptr,
+                           mx_use_tiles(T, F, clt_ceil_div(d, 32)) && mx_tiles_fit(F, pre, pre_layer_stride, pre_row_stride, e));
   const size_t need = clt_mx_encode_workspace_bytes(T, d, F, L, x_scales != nullptr);
   if (need > 0 && (!workspace || workspace_bytes < need)) return CLT_ERR_WORKSPACE;
   if (need > 0 && !clt_aligned16(workspace)) return CLT_ERR_ALIGN;
   hipStream_t s = (hipStream_t)stream;
   uint8_t *ws = (uint8_t *)workspace;
-  const uint8_t *xc = (const uint8_t *)x, *xs = x_scales, *wc = (const uint8_t *)w_codes;
+  const void *xc = x;
+  const uint8_t *xs = x_scales, *wc = (const uint8_t *)w_codes;
+  const bool vec = d % 8 == 0 && clt_aligned16(x) && x_layer_stride * e % 16 == 0 && d * e % 16 == 0;
   int rc = CLT_OK;
-  if (!x_scales) {
+  if (!x_scales && p.own_x) {
     const MxRows rows{nullptr, 0, 0, p.xrows, nullptr};
     rc = mx_write(dtype, CLT_MXFP4, x, nullptr, x_layer_stride, d, L, 1, T, d, (uint32_t)p.padded, rows, ws + p.xc, ws + p.xs, p.tiles, s);
     xc = ws + p.xc;
@@ -1047,7 +1171,10 @@ extern "C" int clt_mx_encode(const void *x, const uint8_t *x_scales, const void 
     xs = ws + p.xs;
   }
   if (rc != CLT_OK) return rc;
-  if (dtype == CLT_BF16) return launch_mx_project<bf16_t>(p, xc, xs, wc, w_scales, bias, ws, pre, T, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s);
-  if (dtype == CLT_F16) return launch_mx_project<f16_t>(p, xc, xs, wc, w_scales, bias, ws, pre, T, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s);
-  return launch_mx_project<float>(p, xc, xs, wc, w_scales, bias, ws, pre, T, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s);
+#define CLT_MXE(T_) \
+  launch_mx_project<T_>(p, xc, x_layer_stride, vec, xs, wc, w_scales, bias, ws, pre, T, d, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s)
+  if (dtype == CLT_BF16) return CLT_MXE(bf16_t);
+  if (dtype == CLT_F16) return CLT_MXE(f16_t);
+  return CLT_MXE(float);
+#undef CLT_MXE
 }

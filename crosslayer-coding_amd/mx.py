@@ -51,6 +51,26 @@ def row_layout(width: int, fmt: str) -> Tuple[int, int]:
     return blocks * _BLOCK_BYTES[fmt], blocks
 
 
+class _On:
+    """``torch.cuda.device(device)``, which costs more than a launch, where the device is not the current one."""
+
+    __slots__ = ("index", "back")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        current = torch._C._cuda_getDevice()
+        self.back = current if self.index is not None and self.index != current else None
+        if self.back is not None:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.back is not None:
+            torch.cuda.set_device(self.back)
+        return False
+
+
 def _check_values(t: torch.Tensor, what: str) -> None:
     if t.dtype not in _FLOATS:
         raise ValueError(f"{what}: float32, bfloat16 or float16 is taken, got {t.dtype}")
@@ -109,7 +129,7 @@ class MXTensor:
             raise ValueError(f"out must be contiguous {tuple(self.shape)} on {self.device}")
         if out.dtype not in _FLOATS:
             raise ValueError(f"float32, bfloat16 or float16 is given, got {out.dtype}")
-        with torch.cuda.device(self.device):
+        with _On(self.device):
             code = nat.load().clt_mx_dequantise(nat.ptr(self.codes), nat.ptr(self.scales), out.numel() // self.width, self.width,
                                                 FORMATS[self.fmt], nat.ptr(out), self.width, nat.dtype_code(out.dtype),
                                                 nat.current_stream(self.device))
@@ -135,7 +155,7 @@ def quantise(x: torch.Tensor, fmt: str = "mxfp4", out: Optional[MXTensor] = None
     rows = _rows_2d(x)
     if rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]:
         rows = rows.contiguous()                    # an expanded tensor
-    with torch.cuda.device(x.device):
+    with _On(x.device):
         code = nat.load().clt_mx_quantise(nat.ptr(rows), rows.shape[0], rows.shape[1], rows.stride(0), nat.dtype_code(x.dtype),
                                           FORMATS[fmt], nat.ptr(out.codes), nat.ptr(out.scales), nat.current_stream(x.device))
     nat.check(code, "clt_mx_quantise")
@@ -150,10 +170,12 @@ def project(x: Union[torch.Tensor, MXTensor], w: MXTensor, b: Optional[torch.Ten
     `engine.Workspace` to take the scratch memory from."""
     if w.fmt != "mxfp4" or len(w.shape) not in (2, 3):
         raise ValueError(f"the weights must be mxfp4 [L, F, d] or [F, d], got {w.fmt} {tuple(w.shape)}")
-    if len(x.shape) != len(w.shape) or x.shape[-1] != w.width or x.shape[:-2] != w.shape[:-2]:
-        raise ValueError(f"x {tuple(x.shape)} and weights {tuple(w.shape)} do not belong together")
-    if x.device != w.device:
-        raise ValueError(f"x is on {x.device}, the weights are on {w.device}")
+    w_shape, x_shape = w.shape, x.shape
+    if len(x_shape) != len(w_shape) or x_shape[-1] != w.width or x_shape[:-2] != w_shape[:-2]:
+        raise ValueError(f"x {tuple(x_shape)} and weights {tuple(w_shape)} do not belong together")
+    device = w.codes.device
+    if x.device != device:
+        raise ValueError(f"x is on {x.device}, the weights are on {device}")
     if isinstance(x, MXTensor):
         if x.fmt != "mxfp4":
             raise ValueError(f"x must be mxfp4, got {x.fmt}")
@@ -166,15 +188,15 @@ def project(x: Union[torch.Tensor, MXTensor], w: MXTensor, b: Optional[torch.Ten
         dtype = x.dtype
     if dtype not in _FLOATS:
         raise ValueError(f"float32, bfloat16 or float16 is given, got {dtype}")
-    shape = (*x.shape[:-1], w.shape[-2])
-    if b is not None and (b.shape != (*w.shape[:-2], w.shape[-2]) or b.dtype != dtype or b.device != w.device):
-        raise ValueError(f"the bias must be {dtype} {(*w.shape[:-2], w.shape[-2])} on {w.device}, got {b.dtype} {tuple(b.shape)} on {b.device}")
+    shape = (*x_shape[:-1], w_shape[-2])
+    if b is not None and (b.shape != w_shape[:-1] or b.dtype != dtype or b.device != device):
+        raise ValueError(f"the bias must be {dtype} {tuple(w_shape[:-1])} on {device}, got {b.dtype} {tuple(b.shape)} on {b.device}")
     if b is not None and b.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("project has no gradient: call it under torch.no_grad() or on detached tensors")
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=w.device)
-    elif out.shape != shape or out.dtype != dtype or out.device != w.device or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous {dtype} {shape} on {w.device}")
+        out = torch.empty(shape, dtype=dtype, device=device)
+    elif out.shape != shape or out.dtype != dtype or out.device != device or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {dtype} {shape} on {device}")
     if out.numel() == 0:
         return out
     if b is not None and not b.is_contiguous():
@@ -185,15 +207,12 @@ def project(x: Union[torch.Tensor, MXTensor], w: MXTensor, b: Optional[torch.Ten
     T, F = shape[-2], shape[-1]
     L = shape[0] if len(shape) == 3 else 1
     lib = nat.load()
-    with torch.cuda.device(w.device):
+    with _On(device):
         nbytes = lib.clt_mx_encode_workspace_bytes(T, w.width, F, L, int(given))
-        if ws is not None:
-            scratch = ws.get("mx_project", nbytes)
-        else:
-            scratch = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
+        scratch = None if nbytes == 0 else ws.get("mx_project", nbytes) if ws is not None else torch.empty(nbytes, dtype=torch.uint8, device=device)
         code = lib.clt_mx_encode(nat.ptr(x.codes if given else x), nat.ptr(x.scales if given else None), nat.ptr(w.codes), nat.ptr(w.scales),
                                  nat.ptr(b), nat.ptr(out), T, w.width, F, L, T * w.width, F, T * F, F, nat.dtype_code(dtype),
-                                 nat.ptr(scratch), scratch.numel(), nat.current_stream(w.device))
+                                 nat.ptr(scratch), nbytes, nat.current_stream(device))
     nat.check(code, "clt_mx_encode")
     return out
 
@@ -217,7 +236,7 @@ class MXActivationCache:
         held = MXTensor(codes, scales, fmt, d_model)
         if codes.dim() != 4 or codes.shape[1] != 2 or codes.shape[0] < 1:
             raise ValueError(f"codes must be [layers, 2, rows, bytes], got {tuple(codes.shape)}")
-        self._held = held
+        self.codes, self.scales, self.device = held.codes, held.scales, held.codes.device
         self.num_layers, _, self.rows, _ = codes.shape
         if self.rows > 2 ** 31 - 1:
             raise ValueError("a cache holds at most 2^31 - 1 rows")
@@ -233,20 +252,8 @@ class MXActivationCache:
                    torch.full((num_layers, 2, rows, blocks), 255, dtype=torch.uint8, device=device), fmt, d_model)
 
     @property
-    def codes(self) -> torch.Tensor:
-        return self._held.codes
-
-    @property
-    def scales(self) -> torch.Tensor:
-        return self._held.scales
-
-    @property
-    def device(self) -> torch.device:
-        return self._held.device
-
-    @property
     def nbytes(self) -> int:
-        return self._held.nbytes
+        return self.codes.numel() + self.scales.numel()
 
     def _resolve(self, rows: Rows) -> Tuple[Optional[torch.Tensor], int, int]:
         """(row numbers on the device or None, first row, number of rows)."""
@@ -308,7 +315,7 @@ class MXActivationCache:
             if self._owner is None:
                 self._owner = torch.empty(self.rows, dtype=torch.int32, device=self.device)
             owner = self._owner
-        with torch.cuda.device(self.device):
+        with _On(self.device):
             code = nat.load().clt_mx_cache_write(
                 nat.ptr(x), nat.ptr(tg), x.stride(0), row_stride, nat.dtype_code(x.dtype), nat.ptr(index),
                 0 if index is None else 8 * index.element_size(), first, n, self.d_model, self.num_layers, FORMATS[self.fmt],
@@ -350,7 +357,7 @@ class MXActivationCache:
             held = tuple(tables)
         if n == 0:
             return out[0], out[1]
-        with torch.cuda.device(self.device):
+        with _On(self.device):
             code = nat.load().clt_mx_cache_read(
                 nat.ptr(self.codes), nat.ptr(self.scales), self.rows, FORMATS[self.fmt], nat.ptr(index),
                 0 if index is None else 8 * index.element_size(), first, n, d, L, _NORM_MODES[normalization],

@@ -128,13 +128,13 @@ def test_library_refuses_before_it_launches():
     assert r(p, p, 8, 0, None, 0, 0, 4, 64, 1, 0, None, None, None, None, 1.0, p, p, 1, 4, 0, None) == -1
     assert r(p, p, 0, 0, p, 32, 0, 4, 64, 1, 0, None, None, None, None, 1.0, p, p, 0, 4, 0, None) == -1
     e = lib.clt_mx_encode
-    ws = lib.clt_mx_encode_workspace_bytes(4, 64, 16, 1, 0)
-    assert ws >= 4 * 34 and lib.clt_mx_encode_workspace_bytes(4, 64, 16, 1, 1) == 0
+    ws = lib.clt_mx_encode_workspace_bytes(400, 64, 512, 1, 0)
+    assert ws >= 400 * 34 and lib.clt_mx_encode_workspace_bytes(4, 64, 16, 1, 1) == 0
     assert lib.clt_mx_encode_workspace_bytes(0, 64, 16, 1, 0) == 0 and lib.clt_mx_encode_workspace_bytes(4, 262145, 16, 1, 0) == 0
     assert e(p, None, p, p, None, p, 4, 64, 16, 1, 256, 0, 64, 15, 0, p, ws, None) == -1
     assert e(p, None, p, p, None, p, 4, 64, 16, 1, 256, 0, 64, 16, 5, p, ws, None) == -2
-    assert e(p, None, p, p, None, p, 4, 64, 16, 1, 256, 0, 64, 16, 0, p, ws - 1, None) == -3
-    assert e(p, None, p, p, None, p, 4, 64, 16, 1, 256, 0, 64, 16, 0, None, ws, None) == -3
+    assert e(p, None, p, p, None, p, 400, 64, 512, 1, 25600, 0, 204800, 512, 0, p, ws - 1, None) == -3
+    assert e(p, None, p, p, None, p, 400, 64, 512, 1, 25600, 0, 204800, 512, 0, None, ws, None) == -3
     assert e(p, None, p + 8, p, None, p, 4, 64, 16, 1, 256, 0, 64, 16, 0, p, ws, None) == -5
     assert e(None, None, None, None, None, None, 0, 64, 16, 1, 0, 0, 64, 16, 0, None, 0, None) == 0
     assert e(p, None, p, p, None, p, 2 ** 20 + 1, 64, 16, 1, 256, 0, 64, 16, 0, p, ws, None) == -6
