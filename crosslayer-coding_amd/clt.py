@@ -222,6 +222,23 @@ class CrossLayerTranscoder(BaseTranscoder):
             raise AttributeError("ThetaManager is not initialised; cannot set log_threshold.")
         self.theta_manager.log_threshold = new_param
 
+    # ---- 4-bit encoder -------------------------------------------------------------------------
+    def quantise_encoder(self, fmt: str = "mxfp4") -> None:
+        """Compute pre-activations from 4-bit weights and inputs from here on (inference: forward, activations, evaluation, theta
+        estimation).  The parameters and checkpoints stay as they are, and what is written to them shows in the next forward;
+        ``dequantise_encoder()`` goes back.  Selection and decode are the same; training entry points raise meanwhile."""
+        self._sync_device()
+        self.encoder_module.quantise(fmt)
+
+    def dequantise_encoder(self) -> None:
+        """Undo ``quantise_encoder``."""
+        self.encoder_module.dequantise()
+
+    def _no_quantised(self, what: str) -> None:
+        if self.encoder_module.quantised:
+            raise NotImplementedError(f"{what}: the encoder is quantised ({self.encoder_module.quantised}), which is for inference; "
+                                      "call dequantise_encoder() first")
+
     @torch.no_grad()
     def estimate_theta_posthoc(self, data_iter, num_batches: Optional[int] = None, default_theta_value: float = 1e6,
                                device: Optional[torch.device] = None) -> torch.Tensor:
@@ -272,6 +289,7 @@ class CrossLayerTranscoder(BaseTranscoder):
         """(per-layer losses [L] fp32, raw gradients): ``enc_w`` [L, F, d], ``enc_b`` [L, F],
         ``dec_w`` [n_dec, F, d] (feature-major, decoders in slot order: "s->t" pairs, or one per source /
         per target for tied decoders), ``dec_b`` [n_dec, d] (bias gradient of each decoder); all fp32."""
+        self._no_quantised("loss_and_gradients")
         cfg = self.config
         L, d, F = cfg.num_layers, cfg.d_model, cfg.num_features
         if sorted(inputs) != list(range(L)) or sorted(targets) != list(range(L)):
@@ -656,7 +674,8 @@ class CrossLayerTranscoder(BaseTranscoder):
         if prep is None:
             return None
         _, x_slab, w_slab, b_slab = prep
-        if fn == "batchtopk" and cfg.topk_mode == "per_layer" and self.fuse_encode_select:
+        fused = self.fuse_encode_select and not self.encoder_module.quantised
+        if fn == "batchtopk" and cfg.topk_mode == "per_layer" and fused:
             # the encoder keeps only the candidates above a sampled cut; nothing dense is written
             k = int(cfg.batchtopk_k)
             if engine.encode_collect_supported(x_slab, w_slab, b_slab, k):
@@ -666,7 +685,7 @@ class CrossLayerTranscoder(BaseTranscoder):
                 return layers, T, surv
         if fn in ("jumprelu", "relu"):
             return layers, T, self._threshold_survivors(fn, layers, T, x_slab, w_slab, b_slab, pre_buf, ws)
-        pre = engine.encode(x_slab, w_slab, b_slab, out=pre_buf)
+        pre = self.encoder_module.project(layers, x_slab, w_slab, b_slab, out=pre_buf, ws=ws)
         if fn in ("batchtopk", "topk"):
             surv = self._select(pre)
         else:
@@ -727,14 +746,14 @@ class CrossLayerTranscoder(BaseTranscoder):
                 theta = theta.index_select(0, torch.tensor(layers, device=theta.device)).contiguous()
         read_back = pre_buf is None or self._threshold_reads_back(n, T, F)
         surv = None
-        if fn == "jumprelu" and self.fuse_encode_select:
+        if fn == "jumprelu" and self.fuse_encode_select and not self.encoder_module.quantised:
             # thresholds applied in the encoder epilogue; the pool is sized from the density seen so far
             surv = engine.encode_threshold(x_slab, w_slab, b_slab, theta, ws, self._density_ppm,
                                            pre_scratch=None if read_back else pre_buf)
             if surv is None and read_back:
                 self._density_ppm = min(1000000, 4 * self._density_ppm)
         if surv is None:
-            pre = engine.encode(x_slab, w_slab, b_slab, out=pre_buf)
+            pre = self.encoder_module.project(layers, x_slab, w_slab, b_slab, out=pre_buf, ws=ws)
             surv = engine.threshold_select(pre, theta, nat.PRED_GE_THETA if fn == "jumprelu" else nat.PRED_GT_ZERO, ws,
                                            read_back=read_back)
         if surv.status is None:
@@ -880,7 +899,8 @@ class CrossLayerTranscoder(BaseTranscoder):
         layers, x_slab, w_slab, b_slab = prep
         if x_slab.shape[1] != T:
             return None
-        pre = engine.encode(x_slab, w_slab, b_slab, out=self._workspace().typed(buffer, (n, T, F), self.dtype))
+        pre = self.encoder_module.project(layers, x_slab, w_slab, b_slab, out=self._workspace().typed(buffer, (n, T, F), self.dtype),
+                                          ws=self._workspace())
         theta = None
         if fn == "jumprelu":
             theta = self.theta_manager.thresholds(self.dtype)
@@ -949,13 +969,14 @@ class CrossLayerTranscoder(BaseTranscoder):
         if torch.is_grad_enabled() and self.dtype != torch.float16:
             named = list(self.named_parameters())
             if any(p.requires_grad for _, p in named):
-                if self._graph_route_ok(inputs):
+                if self._graph_route_ok(inputs) and not self.encoder_module.quantised:
                     outs = _ReconstructionsWithGraph.apply(self, inputs, [n for n, _ in named], *[p for _, p in named])
                     return {l: outs[l] for l in range(L)}
                 if not getattr(self, "_warned_no_graph", False):
                     self._warned_no_graph = True
                     logger.warning(f"Rank {self.rank}: forward builds no autograd graph for these inputs (it needs one "
-                                   f"2-D or 3-D tensor per layer with equal token counts); gradients will not flow.")
+                                   f"2-D or 3-D tensor per layer with equal token counts, and an encoder that is not quantised); "
+                                   f"gradients will not flow.")
         dense = self._forward_dense_thresholds(inputs)
         if dense is not None:
             return dense

@@ -163,10 +163,11 @@ template <typename T, int FMT, bool VEC>
 __global__ __launch_bounds__(MX_THREADS) void k_mx_write(const T *__restrict__ src0, const T *__restrict__ src1, int64_t layer_stride,
                                                          int64_t row_stride, int kinds, int64_t n, int64_t d, uint32_t blocks,
                                                          uint32_t magic, MxRows rows, uint8_t *__restrict__ codes,
-                                                         uint8_t *__restrict__ scales, int tiled) {
+                                                         uint8_t *__restrict__ scales, int tiled, const int32_t *__restrict__ gate) {
   const MxPiece at = mx_piece(blocks * 2u, magic);
   if (at.j >= n) return;                               // whole pairs: a row has whole blocks
   const int64_t l = blockIdx.y / (uint32_t)kinds;
+  if (gate && gate[l] == 0) return;                    // layers that did not ask for it stay as they are
   const int kind = (int)(blockIdx.y - (uint32_t)l * (uint32_t)kinds);
   const int64_t c = (int64_t)at.p * 16;
   const T *sp = (kind ? src1 : src0) + l * layer_stride + at.j * row_stride + c;
@@ -875,7 +876,7 @@ uint32_t mx_magic(uint32_t pieces) { return (uint32_t)((0x100000000ull + pieces 
 
 template <typename T, int FMT>
 int launch_mx_write(const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t L, int kinds, int64_t n, int64_t d,
-                    uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, hipStream_t s) {
+                    uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, const int32_t *gate, hipStream_t s) {
   const uint32_t pieces = blocks * 2;
   const int64_t groups = clt_ceil_div(n * (int64_t)pieces, MX_THREADS);
   if (groups > 2147483647LL) return CLT_ERR_RANGE;
@@ -884,7 +885,7 @@ int launch_mx_write(const void *src0, const void *src1, int64_t layer_stride, in
   const dim3 grid((unsigned)groups, (unsigned)(L * kinds));
 #define CLT_MXW(VEC)                                                                                                               \
   k_mx_write<T, FMT, VEC><<<grid, MX_THREADS, 0, s>>>((const T *)src0, (const T *)src1, layer_stride, row_stride, kinds, n, d, blocks, \
-                                                      mx_magic(pieces), rows, (uint8_t *)codes, scales, tiled)
+                                                      mx_magic(pieces), rows, (uint8_t *)codes, scales, tiled, gate)
   if (vec) CLT_MXW(true);
   else CLT_MXW(false);
 #undef CLT_MXW
@@ -893,17 +894,17 @@ int launch_mx_write(const void *src0, const void *src1, int64_t layer_stride, in
 
 template <typename T>
 int mx_write_as(int fmt, const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t L, int kinds, int64_t n,
-                int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, hipStream_t s) {
-  if (fmt == CLT_MXFP4) return launch_mx_write<T, CLT_MXFP4>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
-  if (fmt == CLT_MXFP8) return launch_mx_write<T, CLT_MXFP8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
-  return launch_mx_write<T, CLT_MXINT8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
+                int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, const int32_t *gate, hipStream_t s) {
+  if (fmt == CLT_MXFP4) return launch_mx_write<T, CLT_MXFP4>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, gate, s);
+  if (fmt == CLT_MXFP8) return launch_mx_write<T, CLT_MXFP8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, gate, s);
+  return launch_mx_write<T, CLT_MXINT8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, gate, s);
 }
 
 int mx_write(int dtype, int fmt, const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t L, int kinds,
-             int64_t n, int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, hipStream_t s) {
-  if (dtype == CLT_BF16) return mx_write_as<bf16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
-  if (dtype == CLT_F16) return mx_write_as<f16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
-  return mx_write_as<float>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
+             int64_t n, int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, const int32_t *gate, hipStream_t s) {
+  if (dtype == CLT_BF16) return mx_write_as<bf16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, gate, s);
+  if (dtype == CLT_F16) return mx_write_as<f16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, gate, s);
+  return mx_write_as<float>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, gate, s);
 }
 
 template <typename OutT, int FMT>
@@ -1071,7 +1072,20 @@ extern "C" int clt_mx_quantise(const void *src, int64_t n, int64_t d, int64_t ro
   if (!src || !codes || !scales || (n > 1 && row_stride < d)) return CLT_ERR_ARG;
   if (!clt_aligned16(codes)) return CLT_ERR_ALIGN;
   const MxRows rows{nullptr, 0, 0, n, nullptr};
-  return mx_write(dtype, fmt, src, nullptr, 0, row_stride, 1, 1, n, d, (uint32_t)clt_ceil_div(d, 32), rows, codes, scales, 0, (hipStream_t)stream);
+  return mx_write(dtype, fmt, src, nullptr, 0, row_stride, 1, 1, n, d, (uint32_t)clt_ceil_div(d, 32), rows, codes, scales, 0, nullptr, (hipStream_t)stream);
+}
+
+extern "C" int clt_mx_quantise_if(const void *src, int64_t L, int64_t n, int64_t d, int64_t layer_stride, int dtype, int fmt, void *codes,
+                                  uint8_t *scales, const int32_t *changed, void *stream) {
+  if (!clt_model_dtype(dtype)) return CLT_ERR_DTYPE;
+  if (!mx_format(fmt)) return CLT_ERR_ARG;
+  if (const int rc = mx_sizes(L, n, d, n)) return rc;
+  if (n == 0) return CLT_OK;
+  if (!src || !codes || !scales || !changed || layer_stride < 0) return CLT_ERR_ARG;
+  if (!clt_aligned16(codes)) return CLT_ERR_ALIGN;
+  const MxRows rows{nullptr, 0, 0, n, nullptr};
+  return mx_write(dtype, fmt, src, nullptr, layer_stride, d, L, 1, n, d, (uint32_t)clt_ceil_div(d, 32), rows, codes, scales, 0, changed,
+                  (hipStream_t)stream);
 }
 
 extern "C" int clt_mx_dequantise(const void *codes, const uint8_t *scales, int64_t n, int64_t d, int fmt, void *dst, int64_t row_stride,
@@ -1104,7 +1118,7 @@ extern "C" int clt_mx_cache_write(const void *x, const void *tgt, int64_t layer_
     k_mx_claim<<<nb, 256, 0, s>>>(r, n, owner, 0);
     k_mx_claim<<<nb, 256, 0, s>>>(r, n, owner, 1);
   }
-  return mx_write(dtype, fmt, x, tgt, layer_stride, row_stride, L, 2, n, d, (uint32_t)clt_ceil_div(d, 32), r, codes, scales, 0, s);
+  return mx_write(dtype, fmt, x, tgt, layer_stride, row_stride, L, 2, n, d, (uint32_t)clt_ceil_div(d, 32), r, codes, scales, 0, nullptr, s);
 }
 
 extern "C" int clt_mx_cache_read(const void *codes, const uint8_t *scales, int64_t rows, int fmt, const void *row_index, int index_bits,
@@ -1158,7 +1172,7 @@ extern "C" int clt_mx_encode(const void *x, const uint8_t *x_scales, const void 
   int rc = CLT_OK;
   if (!x_scales && p.own_x) {
     const MxRows rows{nullptr, 0, 0, p.xrows, nullptr};
-    rc = mx_write(dtype, CLT_MXFP4, x, nullptr, x_layer_stride, d, L, 1, T, d, (uint32_t)p.padded, rows, ws + p.xc, ws + p.xs, p.tiles, s);
+    rc = mx_write(dtype, CLT_MXFP4, x, nullptr, x_layer_stride, d, L, 1, T, d, (uint32_t)p.padded, rows, ws + p.xc, ws + p.xs, p.tiles, nullptr, s);
     xc = ws + p.xc;
     xs = ws + p.xs;
   } else if (p.tiles) {

@@ -15,7 +15,8 @@ from typing import Dict, List, Optional, Tuple
 import torch
 import torch.nn as nn
 
-from . import engine
+from . import _native as nat
+from . import engine, mx
 from .parallel import ColumnParallelLinear, own_parameter, require_single_rank
 
 logger = logging.getLogger(__name__)
@@ -37,6 +38,12 @@ class Encoder(nn.Module):
             ColumnParallelLinear(d, F, bias=True, process_group=process_group, device=device, dtype=dtype,
                                  weight_storage=self._w_slab[l], bias_storage=self._b_slab[l])
             for l in range(L))
+        # 4-bit copy of the weights (`quantise`), the parameters it was made from, and the fingerprints of their data
+        self._mx: Optional[mx.MXTensor] = None
+        self._mx_keys: Optional[Tuple] = None
+        self._mx_state: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]] = None
+        self._mx_fmt: Optional[str] = None
+        self.watch_parameter_data = True
 
     # ---- slab bookkeeping -------------------------------------------------------
     def first_weight(self) -> torch.Tensor:
@@ -70,6 +77,62 @@ class Encoder(nn.Module):
             self._w_slab, self._b_slab = w, b
             self.device, self.dtype = w.device, w.dtype
         return self._w_slab, self._b_slab
+
+    # ---- 4-bit weights --------------------------------------------------------------
+    @property
+    def quantised(self) -> Optional[str]:
+        """Format of the weights that the projection multiplies, None while these are the parameters themselves."""
+        return self._mx_fmt
+
+    def quantise(self, fmt: str = "mxfp4") -> None:
+        """Project from a 4-bit copy of the weights from here on (`mx.project`); the parameters stay as they are."""
+        if fmt != "mxfp4":
+            raise ValueError(f"the projection takes mxfp4 weights, asked for {fmt!r}")
+        nat.require_device(self.first_weight(), "quantise")
+        mx.row_layout(self.config.d_model, fmt)
+        self._mx_fmt = fmt
+        self.quantised_weights()
+
+    def dequantise(self) -> None:
+        """Project from the parameters again; the copy is given back."""
+        self._mx_fmt, self._mx, self._mx_keys, self._mx_state = None, None, None, None
+
+    def quantised_weights(self) -> mx.MXTensor:
+        """The copy, true to the parameters: made anew where a parameter's storage or version counter changed, and by the
+        device itself for layers whose data alone did (``weight.data.fill_(...)``: every row and column of a weight is looked
+        at; ``watch_parameter_data`` = False leaves that out)."""
+        w, _ = self.stacked()
+        L, F, d = w.shape
+        weights = [own_parameter(enc, "weight") for enc in self.encoders._modules.values()]
+        keys = tuple((p.data_ptr(), p._version) for p in weights)
+        if self._mx is None or self._mx.device != w.device or self._mx_keys != keys:
+            out = self._mx if self._mx is not None and self._mx.device == w.device and self._mx.shape == w.shape else None
+            with torch.no_grad():
+                self._mx = mx.quantise(w.detach(), self._mx_fmt, out=out)
+            self._mx_keys = keys
+            self._mx_state = None
+        if self.watch_parameter_data:
+            fresh = self._mx_state is None
+            if fresh:
+                host = torch.tensor([k[0] for k in keys], dtype=torch.int64).pin_memory()
+                self._mx_state = (host.to(w.device, non_blocking=True), torch.zeros(16 * L, dtype=torch.int64, device=w.device),
+                                  torch.zeros(L, dtype=torch.int32, device=w.device), host)
+            table, state, changed, _ = self._mx_state
+            engine.decoder_fingerprint(table, F, d, w.dtype, state, changed, fresh)
+            if not fresh:
+                mx.quantise_if(w.detach(), self._mx, changed)
+        return self._mx
+
+    def project(self, layers: List[int], x: torch.Tensor, w: torch.Tensor, b: torch.Tensor, out: Optional[torch.Tensor] = None,
+                ws: Optional[engine.Workspace] = None) -> torch.Tensor:
+        """Pre-activations of ``prepare_slab``'s (layers, x, w, b), from the 4-bit weights where there are some."""
+        if self._mx_fmt is None:
+            return engine.encode(x, w, b, out=out)
+        q = self.quantised_weights()
+        if layers != list(range(self.config.num_layers)):
+            q = q.index_select(torch.tensor(layers, device=w.device))
+        with torch.no_grad():
+            return mx.project(x, q, b.detach(), out=out, ws=ws)
 
     # ---- reference interface ------------------------------------------------------
     def _zeros(self, rows: int) -> torch.Tensor:
@@ -111,7 +174,7 @@ class Encoder(nn.Module):
             return self._zeros(rows)
         w, b = self.stacked()
         l = layer_idx % len(self.encoders)
-        return engine.encode(flat.detach().contiguous().unsqueeze(0), w[l:l + 1], b[l:l + 1])[0]
+        return self.project([l], flat.detach().contiguous().unsqueeze(0), w[l:l + 1], b[l:l + 1])[0]
 
     def encode_all_layers(self, inputs: Dict[int, torch.Tensor]
                           ) -> Tuple[Dict[int, torch.Tensor], List[Tuple[int, int, int]]]:
@@ -138,7 +201,7 @@ class Encoder(nn.Module):
         if prep is None:
             return None
         layers, x_slab, ws, bs = prep
-        return layers, engine.encode(x_slab, ws, bs, out=out)
+        return layers, self.project(layers, x_slab, ws, bs, out=out)
 
     def prepare_slab(self, inputs: Dict[int, torch.Tensor]):
         """(sorted layers, x [n, T, d], weights [n, F, d], biases [n, F]) of the given layers, or

@@ -13,7 +13,9 @@ the file / HTTP transport left to the caller:
   Every chunk of a batch is one `clt_feed_gather` launch that writes all layers, inputs and
   targets into two ``[L, T, d]`` slabs - no per-layer tensors, no ``torch.cat``, no fp32 copy.
   Chunks can be made resident (288 GB of HBM hold whole datasets; pinned host memory works too,
-  the kernel reads it in place) or arrive per batch as the bytes of ``_fetch_slice``.
+  the kernel reads it in place) or arrive per batch as the bytes of ``_fetch_slice``.  Resident chunks may be held in a
+  microscaled format (``store="mxfp8"``, "mxint8" or "mxfp4": `mx.MXActivationCache`), quantised as they are added or, row by
+  row, as they are harvested (`open_chunk`, `write_rows`), and expanded as a batch is drawn.
 """
 
 from __future__ import annotations
@@ -27,6 +29,7 @@ import numpy as np
 import torch
 
 from . import _native as nat
+from . import mx
 
 logger = logging.getLogger(__name__)
 
@@ -115,11 +118,13 @@ def prepare_normalization(norm_stats: Optional[Dict[str, Any]], layer_indices: L
 
 
 class _Chunk:
-    __slots__ = ("data", "rows", "dtype", "layer_stride", "target_offset")
+    __slots__ = ("data", "rows", "dtype", "layer_stride", "target_offset", "cache")
 
-    def __init__(self, data: torch.Tensor, rows: int, dtype: torch.dtype, layer_stride: int, target_offset: int):
+    def __init__(self, data: Optional[torch.Tensor], rows: int, dtype: torch.dtype, layer_stride: int, target_offset: int,
+                 cache: Optional[mx.MXActivationCache] = None):
         self.data, self.rows, self.dtype = data, rows, dtype
         self.layer_stride, self.target_offset = layer_stride, target_offset
+        self.cache = cache
 
 
 class DeviceActivationFeed:
@@ -162,12 +167,22 @@ class DeviceActivationFeed:
 
     # ---- resident chunks ----
     def add_chunk(self, chunk_id: int, data: Union[torch.Tensor, np.ndarray, bytes], rows: Optional[int] = None,
-                  where: str = "device") -> None:
+                  where: str = "device", store: Optional[str] = None) -> None:
         """Keep a whole chunk resident.  ``data``: ``[L, 2, rows, d]`` (inputs, targets per layer) as a
         tensor / array of the store dtype, or the same as raw bytes with ``rows`` given.  ``where``:
-        "device" (HBM) or "pinned" (page-locked host memory the kernel reads in place)."""
+        "device" (HBM) or "pinned" (page-locked host memory the kernel reads in place).  ``store``: None keeps
+        the store dtype; "mxfp8", "mxint8" or "mxfp4" quantises the rows into HBM."""
+        if store is not None and where != "device":
+            raise ValueError("a quantised chunk lives in device memory")
         t = self._as_store_tensor(data, rows)
         n = t.shape[2]
+        if store is not None:
+            cache = self._new_cache(n, store)
+            for a in range(0, n, 65536):                # bounds the unquantised copy on the device
+                part = t[:, :, a:a + 65536].to(self.device)
+                cache.write(slice(a, a + part.shape[2]), part[:, 0], part[:, 1])
+            self._chunks[int(chunk_id)] = _Chunk(None, n, self.dtype, 0, 0, cache)
+            return
         if where == "pinned":
             held = torch.empty(t.shape, dtype=t.dtype, pin_memory=True)
             held.copy_(t)
@@ -176,6 +191,27 @@ class DeviceActivationFeed:
         else:
             raise ValueError("where must be 'device' or 'pinned'")
         self._chunks[int(chunk_id)] = _Chunk(held, n, self.dtype, 2 * n * self.d_model, n * self.d_model)
+
+    def _new_cache(self, rows: int, store: str) -> mx.MXActivationCache:
+        if self.device.type != "cuda" or not torch.cuda.is_available():
+            raise nat.CLTNativeError("DeviceActivationFeed: quantised chunks live on a ROCm GPU")
+        return mx.MXActivationCache.empty(self.num_layers, rows, self.d_model, store, self.device)
+
+    def open_chunk(self, chunk_id: int, rows: int, store: str = "mxfp8") -> None:
+        """A resident chunk of ``rows`` rows in a microscaled format, to be filled by `write_rows`; rows read as NaN until
+        they are written."""
+        if rows <= 0:
+            raise ValueError(f"a chunk holds at least one row, got {rows}")
+        self._chunks[int(chunk_id)] = _Chunk(None, rows, self.dtype, 0, 0, self._new_cache(rows, store))
+
+    def write_rows(self, chunk_id: int, rows: mx.Rows, inputs: Union[torch.Tensor, Dict[int, torch.Tensor]],
+                   targets: Union[torch.Tensor, Dict[int, torch.Tensor]]) -> None:
+        """Put a harvest's activations ([L, n, d] or {layer: [n, d]} on the device) into rows of a quantised chunk
+        (`mx.MXActivationCache.write`: a slice, row numbers, or a tensor of them on the device)."""
+        chunk = self._chunks.get(int(chunk_id))
+        if chunk is None or chunk.cache is None:
+            raise ValueError(f"chunk {int(chunk_id)} is not a quantised one: open_chunk or add_chunk(store=...) makes one")
+        chunk.cache.write(rows, inputs, targets)
 
     def _as_store_tensor(self, data, rows: Optional[int]) -> torch.Tensor:
         L, d = self.num_layers, self.d_model
@@ -255,6 +291,11 @@ class DeviceActivationFeed:
         out_row, at = 0, 0
         for chunk, index, raw in pieces:
             n = int(index.shape[0])
+            if chunk is not None and chunk.cache is not None:
+                chunk.cache.read(index_dev[out_row:out_row + n], self.out_dtype, ("none", "mean_std", "sqrt_d_model")[mode],
+                                 self._tables if mode == 1 else None, (x, tg), out_row)
+                out_row += n
+                continue
             if chunk is not None:
                 src_ptr, src_rows = chunk.data.data_ptr(), chunk.rows
                 layer_stride, target_offset = chunk.layer_stride, chunk.target_offset

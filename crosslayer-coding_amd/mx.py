@@ -162,6 +162,22 @@ def quantise(x: torch.Tensor, fmt: str = "mxfp4", out: Optional[MXTensor] = None
     return out
 
 
+def quantise_if(x: torch.Tensor, out: MXTensor, changed: torch.Tensor) -> None:
+    """`quantise` of the layers of ``x`` [L, n, d] whose flag in ``changed`` (int32 [L], on the device) is set, into ``out``."""
+    _check_values(x, "quantise_if")
+    if x.dim() != 3 or out.shape != x.shape or out.device != x.device or x.stride(2) != 1 or x.stride(1) != x.shape[2]:
+        raise ValueError(f"x {tuple(x.shape)} must be rows without gaps, out of its shape: got {tuple(out.shape)}")
+    if changed.dtype != torch.int32 or changed.shape != (x.shape[0],) or changed.device != x.device:
+        raise ValueError(f"changed must be int32 [{x.shape[0]}] on {x.device}")
+    if x.numel() == 0:
+        return
+    with _On(x.device):
+        code = nat.load().clt_mx_quantise_if(nat.ptr(x), x.shape[0], x.shape[1], x.shape[2], x.stride(0), nat.dtype_code(x.dtype),
+                                             FORMATS[out.fmt], nat.ptr(out.codes), nat.ptr(out.scales), nat.ptr(changed),
+                                             nat.current_stream(x.device))
+    nat.check(code, "clt_mx_quantise_if")
+
+
 def project(x: Union[torch.Tensor, MXTensor], w: MXTensor, b: Optional[torch.Tensor] = None,
             out: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None, ws=None) -> torch.Tensor:
     """``pre[l] = x[l] @ w[l].T + b[l]`` on the 4-bit matrix cores: ``w`` [L, F, d] in mxfp4, ``x`` [L, T, d] quantised to

@@ -893,6 +893,8 @@ int clt_feed_gather(const void *src, int src_dtype, int64_t src_rows, int64_t sr
  *
  * clt_mx_quantise / clt_mx_dequantise: n rows of d elements (dtype CLT_F32 / CLT_BF16 / CLT_F16), row_stride elements
  *   apart, to codes and scales and back (fp32, one rounding to dtype).
+ * clt_mx_quantise_if: the same for L layers of n rows (d elements apart; layers layer_stride apart; codes and scales of the
+ *   layers follow one another), those whose flag changed[l] (device) is set: what clt_decoder_fingerprint says of weights.
  *
  * clt_mx_cache_write / clt_mx_cache_read: a store of activations, codes [L][2][rows][row bytes] and scales
  *   [L][2][rows][blocks] (inputs and targets of every layer; clt/training/data/manifest_activation_store.py:555-560 keeps
@@ -918,6 +920,8 @@ int clt_feed_gather(const void *src, int src_dtype, int64_t src_rows, int64_t sr
 int64_t clt_mx_row_bytes(int64_t d, int fmt);
 int clt_mx_quantise(const void *src, int64_t n, int64_t d, int64_t row_stride, int dtype, int fmt,
                     void *codes, uint8_t *scales, void *stream);
+int clt_mx_quantise_if(const void *src, int64_t L, int64_t n, int64_t d, int64_t layer_stride, int dtype,
+                       int fmt, void *codes, uint8_t *scales, const int32_t *changed, void *stream);
 int clt_mx_dequantise(const void *codes, const uint8_t *scales, int64_t n, int64_t d, int fmt,
                       void *dst, int64_t row_stride, int dtype, void *stream);
 int clt_mx_cache_write(const void *x, const void *tgt, int64_t layer_stride, int64_t row_stride,
