@@ -532,6 +532,15 @@ __device__ __forceinline__ void mx_fill16_low(const void *base, uint32_t off, ui
                : "=&s"(all) : "v"(off), "s"(base), "{m0}"(at), "s"(mask) : "memory");
 }
 
+// t / d for t < 2^31 by one product: m = floor(2^(31 + s) / d) + 1 with 2^(s - 1) < d <= 2^s.
+struct MxDiv { uint32_t m; int s; };
+static inline MxDiv mx_div(uint32_t d) {
+  int s = 0;
+  while (((uint64_t)1 << s) < d) ++s;
+  return {s == 0 ? 0u : (uint32_t)(((uint64_t)1 << (31 + s)) / d + 1), s};
+}
+__device__ __forceinline__ int mx_over(int t, const MxDiv &v) { return v.s == 0 ? t : (int)(__umulhi((uint32_t)t, v.m) >> (v.s - 1)); }
+
 struct TileArgs {
   const uint8_t *xc, *wc;                     // x rows hold whole stages (zeros behind the end)
   const uint8_t *xs, *ws;                     // [L][tiles][stages][8 rows of a tile], as the lanes take them (mx_scale_place)
@@ -539,6 +548,7 @@ struct TileArgs {
   int M, xrows, N, tiles_m, tiles_n, total, per_xcd;   // xrows: rows of x per layer that may be read, whole tiles
   int stages, xpitch, wpitch;                 // bytes of a row of codes
   int64_t ps, pre_row;
+  MxDiv per_layer, per_group, last_group, per_stages;   // by tiles of a layer, of 8 feature tiles, by feature tiles of the last group, by stages
 };
 
 template <typename OutT, int MG, bool LINES>
@@ -569,18 +579,17 @@ __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   // K is walked from a stage of the tile's own, so that the CUs that share x or W ask for different lines at any one time.
   struct At { int layer, tm, m0, n0, tn, rot; };
   auto locate = [&](int t) {
-    const int per = a.tiles_m * a.tiles_n;
     At at;
-    at.layer = t / per;
-    t -= at.layer * per;
-    const int g = t / (8 * a.tiles_m), r = t - g * 8 * a.tiles_m;
+    at.layer = mx_over(t, a.per_layer);
+    t -= at.layer * a.tiles_m * a.tiles_n;
+    const int g = mx_over(t, a.per_group), r = t - g * 8 * a.tiles_m;
     const int cnt = min(8, a.tiles_n - g * 8);
-    const int tm = r / cnt;
-    at.tm = tm;
-    at.m0 = tm * BM;
-    at.rot = (int)((unsigned)(3 * tm + min(g * 8 + r - tm * cnt, a.tiles_n - 2)) % (unsigned)a.stages);
-    at.tn = g * 8 + r - tm * cnt;
+    at.tm = cnt == 8 ? r >> 3 : mx_over(r, a.last_group);
+    at.tn = g * 8 + r - at.tm * cnt;
+    at.m0 = at.tm * BM;
     at.n0 = min(at.tn * TN, a.N - TN);
+    const int rot = 3 * at.tm + min(at.tn, a.tiles_n - 2);     // the last tile and its neighbour share features: the same order
+    at.rot = max(rot, 0);
     return at;
   };
   const int step = (int)gridDim.x >> 3;
@@ -597,9 +606,11 @@ __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   // x: rows 8 MG wave + 8 i.  W: row groups in the order of the quarters, first half 0 .. 63 and 128 .. 191, rest behind them
   auto w_row = [&](int i) { const int u = (i & 1) * 8 + wave; return (i >> 1) * 64 + (u >> 3) * 128 + (u & 7) * 8; };
   const uint32_t xo = (uint32_t)(lane >> 3) * (uint32_t)a.xpitch + chunkE, wo = (uint32_t)(lane >> 3) * (uint32_t)a.wpitch;
+  At ahead;                                                    // where the loader is
   auto aim = [&]() {
-    const At at = locate(in_tile);
-    in_stage = at.rot;
+    ahead = locate(in_tile);
+    const At &at = ahead;
+    in_stage = at.rot - mx_over(at.rot, a.per_stages) * a.stages;
     in_x = a.xc + ((int64_t)at.layer * a.xrows + at.m0) * a.xpitch;
     in_w = a.wc + ((int64_t)at.layer * a.N + at.n0) * a.wpitch;
     // eight wavefronts, 64 rows of scales each: those of x, then those of W
@@ -804,12 +815,13 @@ __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const std::true_type yes;
   const std::false_type no;
   int before = 0;
+  At at = ahead;                                               // there are at least two stages: the loader is still in the first tile
   for (;;) {
-    const At at = locate(tile);
-    stage(yes, no, before, at);                                // there are at least two
+    stage(yes, no, before, at);
 #pragma clang loop unroll(disable)
     for (int k = 1; k < a.stages - 1; ++k) stage(no, no, before & (k == 1), at);
     stage(no, yes, before & (a.stages == 2), at);
+    at = ahead;                                                // by now in the next one
     before = 1;
     tile += step;
     if (tile >= last_tile) break;
@@ -1017,7 +1029,8 @@ int launch_mx_project(const MxPlan &p, const void *xc, int64_t x_layer, bool vec
     k_mx_tile_side<OutT, 8><<<dim3((unsigned)p.tn, (unsigned)L), 256, 0, s>>>(wsc, ws + p.ws, (const OutT *)bias, (float *)(ws + p.bias), (int)F,
                                                                               (int)p.blocks, (int)p.stages, bs);
     TileArgs a{(const uint8_t *)xc, wc, xs, ws + p.ws, (const float *)(ws + p.bias), (int)T, (int)p.xrows, (int)F, (int)p.tm, (int)p.tn, (int)total,
-               (int)clt_ceil_div(total, 8), (int)p.stages, (int)p.padded * 16, (int)p.blocks * 16, ps, pre_row};
+               (int)clt_ceil_div(total, 8), (int)p.stages, (int)p.padded * 16, (int)p.blocks * 16, ps, pre_row,
+               mx_div((uint32_t)(p.tm * p.tn)), mx_div((uint32_t)(8 * p.tm)), mx_div((uint32_t)(p.tn % 8 ? p.tn % 8 : 8)), mx_div((uint32_t)p.stages)};
     const int64_t e = sizeof(OutT);
     if (((uintptr_t)pre & 127u) == 0 && pre_row * e % 128 == 0 && ps * e % 128 == 0)
       k_mx_project_tiles<OutT, MX_MG, true><<<grid, TW * 64, 0, s>>>(a, (OutT *)pre);
