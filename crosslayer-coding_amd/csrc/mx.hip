@@ -21,10 +21,10 @@ constexpr int64_t MX_MAX_WIDTH = 262144;    // elements of a row: the pieces of 
 constexpr int MX_MG = 4, MX_BM = 64 * MX_MG, TN = 256, TBLOCKS = 8;
 
 // Where the scale of block b of row r of a tile lies among those of its stage.  The rows of a wavefront are `groups` groups of
-// 16; a lane's bytes are neighbours, ordered by group and block.
+// 16; a word holds a lane's bytes of two groups and both blocks, and the lanes' words are neighbours.
 __host__ __device__ __forceinline__ uint32_t mx_scale_place(uint32_t r, uint32_t b, uint32_t groups) {
   const uint32_t w = r / (16 * groups), i = r / 16 % groups, lane = (b & 3) * 16 + (r & 15);
-  return (w * 64 + lane) * groups * 2 + i * 2 + (b >> 2);
+  return ((w * (groups / 2) + (i >> 1)) * 64 + lane) * 4 + (i & 1) * 2 + (b >> 2);
 }
 
 template <int FMT> struct Mx;
@@ -651,16 +651,16 @@ __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 
   // ---- fragments: row l15 of each group of 16, its blocks lq and lq + 4
   const uint32_t xat = (uint32_t)(wm * 16 * MG + l15) * TROW, wat = (uint32_t)(BM + wn * 128 + l15) * TROW;
-  const uint32_t xsat = (uint32_t)(wm * 64 + lane) * (MG * 2), wsat = (uint32_t)(BM * TBLOCKS + (wn * 64 + lane) * 16);
+  const uint32_t xsat = (uint32_t)(wm * (MG / 2) * 64 + lane) * 4, wsat = (uint32_t)(BM * TBLOCKS + (wn * 4 * 64 + lane) * 4);
   const uint32_t koff[2] = {(uint32_t)(lq ^ ((l15 >> 1) & 7)) * 16u, (uint32_t)((lq + 4) ^ ((l15 >> 1) & 7)) * 16u};
   uint4 fx[MG][2], fw[2][2][2];
   uint32_t sx[MG / 2], sw[2];
   auto read_x = [&](uint32_t buf, int i, int ks) { fx[i][ks] = *reinterpret_cast<const uint4 *>(ring + buf * STAGE + xat + i * 16 * TROW + koff[ks]); };
-  auto read_xs = [&](uint32_t sbuf, int i) { sx[i] = *reinterpret_cast<const uint32_t *>(sring + sbuf * SST + xsat + i * 4); };
+  auto read_xs = [&](uint32_t sbuf, int i) { sx[i] = *reinterpret_cast<const uint32_t *>(sring + sbuf * SST + xsat + i * 256); };
   auto read_w = [&](uint32_t buf, int q, int j, int ks) {
     fw[q & 1][j][ks] = *reinterpret_cast<const uint4 *>(ring + buf * STAGE + wat + (q * 2 + j) * 16 * TROW + koff[ks]);
   };
-  auto read_ws = [&](uint32_t sbuf, int q) { sw[q & 1] = *reinterpret_cast<const uint32_t *>(sring + sbuf * SST + wsat + q * 4); };
+  auto read_ws = [&](uint32_t sbuf, int q) { sw[q & 1] = *reinterpret_cast<const uint32_t *>(sring + sbuf * SST + wsat + q * 256); };
   auto meet = [&]() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -693,16 +693,16 @@ __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     for (int jj = 0; jj < JH; ++jj) {
       const mx_f32x4_t y = acc[i][h * JH + jj];
       if constexpr (sizeof(OutT) == 4) {
-        *reinterpret_cast<mx_f32x4_t *>(park + l15 * 128 + ((jj * 4 + lq) ^ (l15 & 7)) * 16) = y;
+        *reinterpret_cast<mx_f32x4_t *>(park + l15 * 128 + ((jj * 4 + lq) ^ (l15 >> 1)) * 16) = y;
       } else {
-        const int slot = (jj * 2 + (lq >> 1)) ^ (l15 & 7);
+        const int slot = (jj * 2 + (lq >> 1)) ^ (l15 >> 1);
         *reinterpret_cast<uint2 *>(park + l15 * 128 + slot * 16 + (lq & 1) * 8) = make_uint2(mx_pack<OutT>(y[0], y[1]), mx_pack<OutT>(y[2], y[3]));
       }
     }
   };
   typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
   u32x4_t v;
-  auto take = [&](int u) { v = *reinterpret_cast<const u32x4_t *>(park + (u * 8 + (la_out >> 3)) * 128 + (((la_out & 7) ^ (la_out >> 3)) * 16)); };
+  auto take = [&](int u) { v = *reinterpret_cast<const u32x4_t *>(park + (u * 8 + (la_out >> 3)) * 128 + (((la_out & 7) ^ (u * 4 + (la_out >> 4))) * 16)); };
   auto send = [&](int n, int u) {
     const int i = n % MG, h = n / MG;
     const uint32_t out_at = (uint32_t)(wm * 16 * MG + (la_out >> 3)) * out_pitch + (uint32_t)(wn * 128 * (int)sizeof(OutT) + (la_out & 7) * 16);
@@ -839,26 +839,29 @@ __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 }
 
 // What a tile takes beside its codes: the scales of its 256 rows in the lanes' order, zeros where there is no block or no row, and the
-// biases in float32.  grid: x = tiles, y = layers; a thread writes 8 bytes of every stage.
+// biases in float32.  grid: x = tiles, y = layers; a thread writes two words of every stage.
 template <typename T, int GROUPS>
 __global__ __launch_bounds__(256) void k_mx_tile_side(const uint8_t *__restrict__ scales, uint8_t *__restrict__ out, const T *__restrict__ bias,
                                                       float *__restrict__ bias_out, int rows, int blocks, int stages, int64_t bs) {
   const int64_t l = blockIdx.y, tile = l * gridDim.x + blockIdx.x;
   // feature tiles: the last one is moved back inside the matrix
   const int r0 = GROUPS == 8 ? min((int)blockIdx.x * 256, rows - 256) : (int)blockIdx.x * 256;
-  const int at = threadIdx.x * 8, lane = at / (GROUPS * 2) % 64, w = at / (GROUPS * 128), i0 = at % (GROUPS * 2) / 2;
   for (int s = 0; s < stages; ++s) {
-    const int b = s * TBLOCKS + (lane >> 4);
-    uint32_t v[2] = {0u, 0u};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = r0 + (w * GROUPS + i0 + i) * 16 + (lane & 15);
-      if (r < rows) {
-        const uint8_t *p = scales + (l * rows + r) * blocks + b;
-        v[i >> 1] |= ((b < blocks ? (uint32_t)p[0] : 0u) | (b + 4 < blocks ? (uint32_t)p[4] << 8 : 0u)) << ((i & 1) * 16);
+    for (int half = 0; half < 2; ++half) {
+      const int at = half * 256 + threadIdx.x, lane = at % 64, i0 = at / 64 % (GROUPS / 2) * 2, w = at / (32 * GROUPS);
+      const int b = s * TBLOCKS + (lane >> 4);
+      uint32_t v = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = r0 + (w * GROUPS + i0 + i) * 16 + (lane & 15);
+        if (r < rows) {
+          const uint8_t *p = scales + (l * rows + r) * blocks + b;
+          v |= ((b < blocks ? (uint32_t)p[0] : 0u) | (b + 4 < blocks ? (uint32_t)p[4] << 8 : 0u)) << (i * 16);
+        }
       }
+      *reinterpret_cast<uint32_t *>(out + (tile * stages + s) * 2048 + at * 4) = v;
     }
-    *reinterpret_cast<uint2 *>(out + (tile * stages + s) * 2048 + at) = make_uint2(v[0], v[1]);
   }
   if (bias_out) bias_out[tile * 256 + threadIdx.x] = bias ? Elem<T>::to_f32(bias[l * bs + r0 + threadIdx.x]) : 0.0f;
 }
