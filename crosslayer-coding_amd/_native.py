@@ -131,7 +131,7 @@ _SIGNATURES = {
                               _i64, _i64, _int, _vp]),
     "clt_mx_row_bytes": (_i64, [_i64, _int]),
     "clt_mx_quantise": (_int, [_vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp]),
-    "clt_mx_quantise_if": (_int, [_vp, _i64, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _vp]),
+    "clt_mx_refresh": (_int, [_vp, _i64, _i64, _i64, _i64, _int, _vp, _vp, _vp, _vp, _int, _vp]),
     "clt_mx_dequantise": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _i64, _int, _vp]),
     "clt_mx_cache_write": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _int, _i64, _i64, _i64, _i64, _int, _vp, _vp, _i64, _vp, _vp]),
     "clt_mx_cache_read": (_int, [_vp, _vp, _i64, _int, _vp, _int, _i64, _i64, _i64, _i64, _int, _vp, _vp, _vp, _vp, _f64, _vp, _vp,

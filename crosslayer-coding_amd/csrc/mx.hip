@@ -163,11 +163,10 @@ template <typename T, int FMT, bool VEC>
 __global__ __launch_bounds__(MX_THREADS) void k_mx_write(const T *__restrict__ src0, const T *__restrict__ src1, int64_t layer_stride,
                                                          int64_t row_stride, int kinds, int64_t n, int64_t d, uint32_t blocks,
                                                          uint32_t magic, MxRows rows, uint8_t *__restrict__ codes,
-                                                         uint8_t *__restrict__ scales, int tiled, const int32_t *__restrict__ gate) {
+                                                         uint8_t *__restrict__ scales, int tiled) {
   const MxPiece at = mx_piece(blocks * 2u, magic);
   if (at.j >= n) return;                               // whole pairs: a row has whole blocks
   const int64_t l = blockIdx.y / (uint32_t)kinds;
-  if (gate && gate[l] == 0) return;                    // layers that did not ask for it stay as they are
   const int kind = (int)(blockIdx.y - (uint32_t)l * (uint32_t)kinds);
   const int64_t c = (int64_t)at.p * 16;
   const T *sp = (kind ? src1 : src0) + l * layer_stride + at.j * row_stride + c;
@@ -187,6 +186,95 @@ __global__ __launch_bounds__(MX_THREADS) void k_mx_write(const T *__restrict__ s
     if (!tiled) scales[row * blocks + blk] = (uint8_t)s;
     else scales[row / MX_BM * MX_BM * blocks + (blk / 8) * (MX_BM * 8) + mx_scale_place((uint32_t)(row % MX_BM), blk % 8, MX_MG)] = (uint8_t)s;
   }
+}
+
+// ---- weights that may have been written -------------------------------------------------------------------------------
+// Whether rows [L][n][d] still are what their fingerprint says: 64 bytes of every row, at places that go round, so that every row
+// and, from d / 32 rows on (16 bits), every column is looked at.  A layer's sums are of whole numbers, in any order; its last workgroup compares and stores.
+// state: [L][16], a 128-byte line per layer: sum, workgroups that have arrived, fingerprint.
+//
+// 12 x 24576 rows of 768 bf16: 19 MB in 64-byte pieces, 21 us, of a layer's 64 workgroups with six loads in flight a lane; bound by
+// the latency of six rounds.  Eight workgroups a layer, one column a round: 196 us.
+constexpr int WATCH_BLOCKS = 64, WATCH_ROWS = WATCH_BLOCKS * 64;
+template <typename T>
+__global__ __launch_bounds__(256) void k_mx_watch(const T *__restrict__ src, int64_t layer_stride, int64_t n, int64_t d,
+                                                  unsigned long long *__restrict__ state, int32_t *__restrict__ changed, int store_only) {
+  constexpr int PE = 16 / (int)sizeof(T);                  // elements of a lane's piece, a quarter of a row's sample
+  __shared__ unsigned long long part[4];
+  const int64_t l = blockIdx.y;
+  const T *base = src + l * layer_stride;
+  unsigned long long h = 0;
+  const int runs = (int)((d + 4 * PE - 1) / (4 * PE)), step = WATCH_ROWS % runs;
+  int place = (blockIdx.x * 64 + (threadIdx.x >> 2)) % runs;
+#pragma unroll 6
+  for (int64_t r = (int64_t)blockIdx.x * 64 + (threadIdx.x >> 2); r < n; r += WATCH_ROWS) {
+    const int64_t c = (int64_t)place * (4 * PE) + (threadIdx.x & 3) * PE;
+    place += step;
+    if (place >= runs) place -= runs;
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    if (c + PE <= d) __builtin_memcpy(w, base + r * d + c, 16);
+    else {
+      T e[PE] = {};
+#pragma unroll
+      for (int k = 0; k < PE; ++k)
+        if (c + k < d) e[k] = base[r * d + c + k];
+      __builtin_memcpy(w, e, 16);
+    }
+    unsigned long long v = ((unsigned long long)w[1] << 32 | w[0]) * 0x9E3779B97F4A7C15ull ^ (unsigned long long)(r * 4 + (threadIdx.x & 3)) * 0xC2B2AE3D27D4EB4Full;
+    v = (v ^ (v >> 29)) * 0xBF58476D1CE4E5B9ull + ((unsigned long long)w[3] << 32 | w[2]);
+    v = (v ^ (v >> 32)) * 0x94D049BB133111EBull;
+    h += v ^ (v >> 31);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) h += __shfl_xor(h, o);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = h;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  unsigned long long *line = state + l * 16;
+  atomicAdd(line, part[0] + part[1] + part[2] + part[3]);
+  __threadfence();
+  if (atomicAdd(line + 1, 1ull) != (unsigned long long)(gridDim.x - 1)) return;
+  __threadfence();
+  const unsigned long long now = atomicExch(line, 0ull);    // and ready for the next call
+  atomicExch(line + 1, 0ull);
+  changed[l] = !store_only && line[2] != now;
+  line[2] = now;
+}
+
+// mxfp4 rows of the layers that `changed` names; the others cost a launch and no more: 4 us, with a workgroup for every 256 pieces,
+// as a batch is written, 22 us.
+constexpr int REQUANTISE_BLOCKS = 256;
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void k_mx_requantise(const T *__restrict__ src, int64_t layer_stride, int64_t n, int64_t d, int64_t blocks,
+                                                       uint8_t *__restrict__ codes, uint8_t *__restrict__ scales, const int32_t *__restrict__ changed) {
+  const int64_t l = blockIdx.y;
+  if (changed[l] == 0) return;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n * blocks * 2; i += REQUANTISE_BLOCKS * 256) {   // pairs stay together
+    const int64_t j = i / (blocks * 2), p = i - j * blocks * 2, c = p * 16;
+    const T *sp = src + l * layer_stride + j * d + c;
+    float v[16];
+    mx_load8<T, VEC>(sp, d - c, v);
+    mx_load8<T, VEC>(sp + 8, d - c - 8, v + 8);
+    const uint32_t s = mx_scale16<CLT_MXFP4>(v);
+    const uint2 a = mx_encode8<CLT_MXFP4>(*reinterpret_cast<float (*)[8]>(v)), b = mx_encode8<CLT_MXFP4>(*reinterpret_cast<float (*)[8]>(v + 8));
+    const int64_t row = l * n + j;
+    *reinterpret_cast<uint2 *>(codes + row * blocks * 16 + p * 8) = make_uint2(a.x, b.x);
+    if ((p & 1) == 0) scales[row * blocks + (p >> 1)] = (uint8_t)s;
+  }
+}
+
+template <typename T>
+int launch_mx_refresh(const void *src, int64_t layer_stride, int64_t L, int64_t n, int64_t d, void *codes, uint8_t *scales, uint64_t *state,
+                      int32_t *changed, int store_only, hipStream_t s) {
+  k_mx_watch<T><<<dim3(WATCH_BLOCKS, (unsigned)L), 256, 0, s>>>((const T *)src, layer_stride, n, d, (unsigned long long *)state, changed, store_only);
+  if (store_only) return clt_check_launch();
+  const int64_t blocks = clt_ceil_div(d, 32);
+  const dim3 grid(REQUANTISE_BLOCKS, (unsigned)L);
+  if (d % 8 == 0 && clt_aligned16(src) && d * (int64_t)sizeof(T) % 16 == 0 && layer_stride * (int64_t)sizeof(T) % 16 == 0)
+    k_mx_requantise<T, true><<<grid, 256, 0, s>>>((const T *)src, layer_stride, n, d, blocks, (uint8_t *)codes, scales, changed);
+  else
+    k_mx_requantise<T, false><<<grid, 256, 0, s>>>((const T *)src, layer_stride, n, d, blocks, (uint8_t *)codes, scales, changed);
+  return clt_check_launch();
 }
 
 // Which row of the batch a store row keeps when several name it: the last one.  Cleared, then raised: two launches of 1.8 us (one
@@ -891,7 +979,7 @@ uint32_t mx_magic(uint32_t pieces) { return (uint32_t)((0x100000000ull + pieces 
 
 template <typename T, int FMT>
 int launch_mx_write(const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t L, int kinds, int64_t n, int64_t d,
-                    uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, const int32_t *gate, hipStream_t s) {
+                    uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, hipStream_t s) {
   const uint32_t pieces = blocks * 2;
   const int64_t groups = clt_ceil_div(n * (int64_t)pieces, MX_THREADS);
   if (groups > 2147483647LL) return CLT_ERR_RANGE;
@@ -900,7 +988,7 @@ int launch_mx_write(const void *src0, const void *src1, int64_t layer_stride, in
   const dim3 grid((unsigned)groups, (unsigned)(L * kinds));
 #define CLT_MXW(VEC)                                                                                                               \
   k_mx_write<T, FMT, VEC><<<grid, MX_THREADS, 0, s>>>((const T *)src0, (const T *)src1, layer_stride, row_stride, kinds, n, d, blocks, \
-                                                      mx_magic(pieces), rows, (uint8_t *)codes, scales, tiled, gate)
+                                                      mx_magic(pieces), rows, (uint8_t *)codes, scales, tiled)
   if (vec) CLT_MXW(true);
   else CLT_MXW(false);
 #undef CLT_MXW
@@ -909,17 +997,17 @@ int launch_mx_write(const void *src0, const void *src1, int64_t layer_stride, in
 
 template <typename T>
 int mx_write_as(int fmt, const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t L, int kinds, int64_t n,
-                int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, const int32_t *gate, hipStream_t s) {
-  if (fmt == CLT_MXFP4) return launch_mx_write<T, CLT_MXFP4>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, gate, s);
-  if (fmt == CLT_MXFP8) return launch_mx_write<T, CLT_MXFP8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, gate, s);
-  return launch_mx_write<T, CLT_MXINT8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, gate, s);
+                int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, hipStream_t s) {
+  if (fmt == CLT_MXFP4) return launch_mx_write<T, CLT_MXFP4>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
+  if (fmt == CLT_MXFP8) return launch_mx_write<T, CLT_MXFP8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
+  return launch_mx_write<T, CLT_MXINT8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
 }
 
 int mx_write(int dtype, int fmt, const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t L, int kinds,
-             int64_t n, int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, const int32_t *gate, hipStream_t s) {
-  if (dtype == CLT_BF16) return mx_write_as<bf16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, gate, s);
-  if (dtype == CLT_F16) return mx_write_as<f16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, gate, s);
-  return mx_write_as<float>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, gate, s);
+             int64_t n, int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, hipStream_t s) {
+  if (dtype == CLT_BF16) return mx_write_as<bf16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
+  if (dtype == CLT_F16) return mx_write_as<f16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
+  return mx_write_as<float>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
 }
 
 template <typename OutT, int FMT>
@@ -1088,20 +1176,20 @@ extern "C" int clt_mx_quantise(const void *src, int64_t n, int64_t d, int64_t ro
   if (!src || !codes || !scales || (n > 1 && row_stride < d)) return CLT_ERR_ARG;
   if (!clt_aligned16(codes)) return CLT_ERR_ALIGN;
   const MxRows rows{nullptr, 0, 0, n, nullptr};
-  return mx_write(dtype, fmt, src, nullptr, 0, row_stride, 1, 1, n, d, (uint32_t)clt_ceil_div(d, 32), rows, codes, scales, 0, nullptr, (hipStream_t)stream);
+  return mx_write(dtype, fmt, src, nullptr, 0, row_stride, 1, 1, n, d, (uint32_t)clt_ceil_div(d, 32), rows, codes, scales, 0, (hipStream_t)stream);
 }
 
-extern "C" int clt_mx_quantise_if(const void *src, int64_t L, int64_t n, int64_t d, int64_t layer_stride, int dtype, int fmt, void *codes,
-                                  uint8_t *scales, const int32_t *changed, void *stream) {
+extern "C" int clt_mx_refresh(const void *src, int64_t L, int64_t n, int64_t d, int64_t layer_stride, int dtype, void *codes, uint8_t *scales,
+                              uint64_t *state, int32_t *changed, int store_only, void *stream) {
   if (!clt_model_dtype(dtype)) return CLT_ERR_DTYPE;
-  if (!mx_format(fmt)) return CLT_ERR_ARG;
   if (const int rc = mx_sizes(L, n, d, n)) return rc;
   if (n == 0) return CLT_OK;
-  if (!src || !codes || !scales || !changed || layer_stride < 0) return CLT_ERR_ARG;
-  if (!clt_aligned16(codes)) return CLT_ERR_ALIGN;
-  const MxRows rows{nullptr, 0, 0, n, nullptr};
-  return mx_write(dtype, fmt, src, nullptr, layer_stride, d, L, 1, n, d, (uint32_t)clt_ceil_div(d, 32), rows, codes, scales, 0, changed,
-                  (hipStream_t)stream);
+  if (!src || !codes || !scales || !state || !changed || layer_stride < 0) return CLT_ERR_ARG;
+  if (!clt_aligned16(codes) || ((uintptr_t)state & 127u) != 0) return CLT_ERR_ALIGN;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == CLT_BF16) return launch_mx_refresh<bf16_t>(src, layer_stride, L, n, d, codes, scales, state, changed, store_only, s);
+  if (dtype == CLT_F16) return launch_mx_refresh<f16_t>(src, layer_stride, L, n, d, codes, scales, state, changed, store_only, s);
+  return launch_mx_refresh<float>(src, layer_stride, L, n, d, codes, scales, state, changed, store_only, s);
 }
 
 extern "C" int clt_mx_dequantise(const void *codes, const uint8_t *scales, int64_t n, int64_t d, int fmt, void *dst, int64_t row_stride,
@@ -1134,7 +1222,7 @@ extern "C" int clt_mx_cache_write(const void *x, const void *tgt, int64_t layer_
     k_mx_claim<<<nb, 256, 0, s>>>(r, n, owner, 0);
     k_mx_claim<<<nb, 256, 0, s>>>(r, n, owner, 1);
   }
-  return mx_write(dtype, fmt, x, tgt, layer_stride, row_stride, L, 2, n, d, (uint32_t)clt_ceil_div(d, 32), r, codes, scales, 0, nullptr, s);
+  return mx_write(dtype, fmt, x, tgt, layer_stride, row_stride, L, 2, n, d, (uint32_t)clt_ceil_div(d, 32), r, codes, scales, 0, s);
 }
 
 extern "C" int clt_mx_cache_read(const void *codes, const uint8_t *scales, int64_t rows, int fmt, const void *row_index, int index_bits,
@@ -1188,7 +1276,7 @@ extern "C" int clt_mx_encode(const void *x, const uint8_t *x_scales, const void 
   int rc = CLT_OK;
   if (!x_scales && p.own_x) {
     const MxRows rows{nullptr, 0, 0, p.xrows, nullptr};
-    rc = mx_write(dtype, CLT_MXFP4, x, nullptr, x_layer_stride, d, L, 1, T, d, (uint32_t)p.padded, rows, ws + p.xc, ws + p.xs, p.tiles, nullptr, s);
+    rc = mx_write(dtype, CLT_MXFP4, x, nullptr, x_layer_stride, d, L, 1, T, d, (uint32_t)p.padded, rows, ws + p.xc, ws + p.xs, p.tiles, s);
     xc = ws + p.xc;
     xs = ws + p.xs;
   } else if (p.tiles) {

@@ -41,7 +41,7 @@ class Encoder(nn.Module):
         # 4-bit copy of the weights (`quantise`), the parameters it was made from, and the fingerprints of their data
         self._mx: Optional[mx.MXTensor] = None
         self._mx_keys: Optional[Tuple] = None
-        self._mx_state: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]] = None
+        self._mx_state: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
         self._mx_fmt: Optional[str] = None
         self.watch_parameter_data = True
 
@@ -114,13 +114,8 @@ class Encoder(nn.Module):
         if self.watch_parameter_data:
             fresh = self._mx_state is None
             if fresh:
-                host = torch.tensor([k[0] for k in keys], dtype=torch.int64).pin_memory()
-                self._mx_state = (host.to(w.device, non_blocking=True), torch.zeros(16 * L, dtype=torch.int64, device=w.device),
-                                  torch.zeros(L, dtype=torch.int32, device=w.device), host)
-            table, state, changed, _ = self._mx_state
-            engine.decoder_fingerprint(table, F, d, w.dtype, state, changed, fresh)
-            if not fresh:
-                mx.quantise_if(w.detach(), self._mx, changed)
+                self._mx_state = (torch.zeros(16 * L, dtype=torch.int64, device=w.device), torch.zeros(L, dtype=torch.int32, device=w.device))
+            mx.refresh(w.detach(), self._mx, *self._mx_state, store_only=fresh)
         return self._mx
 
     def project(self, layers: List[int], x: torch.Tensor, w: torch.Tensor, b: torch.Tensor, out: Optional[torch.Tensor] = None,

@@ -162,20 +162,26 @@ def quantise(x: torch.Tensor, fmt: str = "mxfp4", out: Optional[MXTensor] = None
     return out
 
 
-def quantise_if(x: torch.Tensor, out: MXTensor, changed: torch.Tensor) -> None:
-    """`quantise` of the layers of ``x`` [L, n, d] whose flag in ``changed`` (int32 [L], on the device) is set, into ``out``."""
-    _check_values(x, "quantise_if")
-    if x.dim() != 3 or out.shape != x.shape or out.device != x.device or x.stride(2) != 1 or x.stride(1) != x.shape[2]:
-        raise ValueError(f"x {tuple(x.shape)} must be rows without gaps, out of its shape: got {tuple(out.shape)}")
-    if changed.dtype != torch.int32 or changed.shape != (x.shape[0],) or changed.device != x.device:
-        raise ValueError(f"changed must be int32 [{x.shape[0]}] on {x.device}")
+def refresh(x: torch.Tensor, out: MXTensor, state: torch.Tensor, changed: torch.Tensor, store_only: bool = False) -> None:
+    """Bring the mxfp4 copy ``out`` of weights ``x`` [L, n, d] up to date where they were written since the last call, decided on the
+    device: fingerprints of every layer (64 bytes of every row) in ``state`` (int64 [16 L], zeros before the first call) are
+    compared, ``changed`` (int32 [L]) says which differ, and those layers are quantised anew.  ``store_only`` records the
+    fingerprints of weights that ``out`` was just made from."""
+    _check_values(x, "refresh")
+    if x.dim() != 3 or out.fmt != "mxfp4" or out.shape != x.shape or out.device != x.device or x.stride(2) != 1 or x.stride(1) != x.shape[2]:
+        raise ValueError(f"x {tuple(x.shape)} must be rows without gaps, out mxfp4 of its shape: got {out.fmt} {tuple(out.shape)}")
+    L = x.shape[0]
+    if state.dtype != torch.int64 or state.shape != (16 * L,) or changed.dtype != torch.int32 or changed.shape != (L,):
+        raise ValueError(f"state must be int64 [{16 * L}], changed int32 [{L}]")
+    if state.device != x.device or changed.device != x.device:
+        raise ValueError(f"state and changed must be on {x.device}")
     if x.numel() == 0:
         return
     with _On(x.device):
-        code = nat.load().clt_mx_quantise_if(nat.ptr(x), x.shape[0], x.shape[1], x.shape[2], x.stride(0), nat.dtype_code(x.dtype),
-                                             FORMATS[out.fmt], nat.ptr(out.codes), nat.ptr(out.scales), nat.ptr(changed),
-                                             nat.current_stream(x.device))
-    nat.check(code, "clt_mx_quantise_if")
+        code = nat.load().clt_mx_refresh(nat.ptr(x), L, x.shape[1], x.shape[2], x.stride(0), nat.dtype_code(x.dtype), nat.ptr(out.codes),
+                                         nat.ptr(out.scales), nat.ptr(state), nat.ptr(changed), 1 if store_only else 0,
+                                         nat.current_stream(x.device))
+    nat.check(code, "clt_mx_refresh")
 
 
 def project(x: Union[torch.Tensor, MXTensor], w: MXTensor, b: Optional[torch.Tensor] = None,

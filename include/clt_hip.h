@@ -893,8 +893,12 @@ int clt_feed_gather(const void *src, int src_dtype, int64_t src_rows, int64_t sr
  *
  * clt_mx_quantise / clt_mx_dequantise: n rows of d elements (dtype CLT_F32 / CLT_BF16 / CLT_F16), row_stride elements
  *   apart, to codes and scales and back (fp32, one rounding to dtype).
- * clt_mx_quantise_if: the same for L layers of n rows (d elements apart; layers layer_stride apart; codes and scales of the
- *   layers follow one another), those whose flag changed[l] (device) is set: what clt_decoder_fingerprint says of weights.
+ * clt_mx_refresh: CLT_MXFP4 codes and scales [L][n] of weights [L][n][d] (rows without gaps, layers layer_stride apart)
+ *   brought up to date where the weights were written.  A fingerprint of every layer - 64 bytes of every row, at places that
+ *   go round - is compared with the one in `state` (uint64 [16 L], 128-byte aligned, zeros before the first call),
+ *   changed[l] (int32 [L]) says where it differs, and those layers are quantised anew.  A write to a matrix, a whole row or
+ *   (n >= d / 16) a whole column shows; one to a few scattered elements may not.  store_only != 0 records the fingerprints
+ *   and quantises nothing.  Calls that share a state are the caller's to order.
  *
  * clt_mx_cache_write / clt_mx_cache_read: a store of activations, codes [L][2][rows][row bytes] and scales
  *   [L][2][rows][blocks] (inputs and targets of every layer; clt/training/data/manifest_activation_store.py:555-560 keeps
@@ -920,8 +924,9 @@ int clt_feed_gather(const void *src, int src_dtype, int64_t src_rows, int64_t sr
 int64_t clt_mx_row_bytes(int64_t d, int fmt);
 int clt_mx_quantise(const void *src, int64_t n, int64_t d, int64_t row_stride, int dtype, int fmt,
                     void *codes, uint8_t *scales, void *stream);
-int clt_mx_quantise_if(const void *src, int64_t L, int64_t n, int64_t d, int64_t layer_stride, int dtype,
-                       int fmt, void *codes, uint8_t *scales, const int32_t *changed, void *stream);
+int clt_mx_refresh(const void *src, int64_t L, int64_t n, int64_t d, int64_t layer_stride, int dtype,
+                   void *codes, uint8_t *scales, uint64_t *state, int32_t *changed, int store_only,
+                   void *stream);
 int clt_mx_dequantise(const void *codes, const uint8_t *scales, int64_t n, int64_t d, int fmt,
                       void *dst, int64_t row_stride, int dtype, void *stream);
 int clt_mx_cache_write(const void *x, const void *tgt, int64_t layer_stride, int64_t row_stride,

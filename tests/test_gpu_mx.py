@@ -425,3 +425,26 @@ def test_captured_and_replayed(dev, T):
         want = _together(other, rows, x, w, b)
         torch.cuda.synchronize()
         assert torch.equal(got, want), trial
+
+
+# ---- weights that were written -----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("L,n,d", [(1, 1, 1), (2, 7, 33), (3, 300, 100), (2, 4100, 256), (2, 130, 2050)])
+def test_refresh_follows_writes_to_any_row_column_or_layer(dev, dtype, L, n, d):
+    g = torch.Generator().manual_seed(n)
+    w = torch.randn(L, n, d, generator=g).to(dtype).to(dev)
+    q = cca.mx.quantise(w)
+    state, changed = torch.zeros(16 * L, dtype=torch.int64, device=dev), torch.zeros(L, dtype=torch.int32, device=dev)
+    cca.mx.refresh(w, q, state, changed, store_only=True)
+    cca.mx.refresh(w, q, state, changed)
+    assert changed.tolist() == [0] * L
+    for trial in range(4):
+        l, r, c = int(torch.randint(L, (1,), generator=g)), int(torch.randint(n, (1,), generator=g)), int(torch.randint(d, (1,), generator=g))
+        for write in (lambda: w[l, r].mul_(-1.5), lambda: w[l, :, c].add_(0.75), lambda: w[l].mul_(0.5)):
+            write()
+            cca.mx.refresh(w, q, state, changed)
+            assert changed.tolist() == [int(i == l) for i in range(L)]
+            _check_codes(q, w.cpu(), "mxfp4")
+            cca.mx.refresh(w, q, state, changed)
+            assert not changed.any()

@@ -138,3 +138,8 @@ def test_library_refuses_before_it_launches():
     assert e(p, None, p + 8, p, None, p, 4, 64, 16, 1, 256, 0, 64, 16, 0, p, ws, None) == -5
     assert e(None, None, None, None, None, None, 0, 64, 16, 1, 0, 0, 64, 16, 0, None, 0, None) == 0
     assert e(p, None, p, p, None, p, 2 ** 20 + 1, 64, 16, 1, 256, 0, 64, 16, 0, p, ws, None) == -6
+    f = lib.clt_mx_refresh
+    assert f(p, 1, 4, 64, 256, 7, p, p, p, p, 0, None) == -2
+    assert f(p, 1, 4, 64, 256, 0, p, p, None, p, 0, None) == -1
+    assert f(p, 1, 4, 64, 256, 0, p, p, p + 64, p, 0, None) == -5
+    assert f(p, 1, 0, 64, 256, 0, None, None, None, None, 0, None) == 0
