@@ -107,7 +107,8 @@ __device__ __forceinline__ int64_t mx_row(const MxRows &r, int64_t j) {
 }
 
 // A workgroup takes 256 neighbouring pieces: row and place in it from 32-bit numbers counted from the group's first row.
-// magic = ceil(2^32 / pieces), exact for counts up to MX_MAX_WIDTH / 4 + 256 (their product with `pieces` stays below 2^32).
+// magic = ceil(2^32 / pieces) = (2^32 + e) / pieces, e < pieces: the quotient of `at` is exact while at * e < 2^32 (pieces - at % pieces),
+// which holds for at < pieces + 256 and pieces <= MX_MAX_WIDTH / 4 = 2^16 (at = pieces - 1 is the tightest).
 // A thread goes on to the same piece of `rows_apart` rows further on, so that several loads are under way and what belongs to
 // the column is fetched once.
 struct MxPiece { int64_t j; uint32_t p; };

@@ -143,3 +143,13 @@ def test_library_refuses_before_it_launches():
     assert f(p, 1, 4, 64, 256, 0, p, p, None, p, 0, None) == -1
     assert f(p, 1, 4, 64, 256, 0, p, p, p + 64, p, 0, None) == -5
     assert f(p, 1, 0, 64, 256, 0, None, None, None, None, 0, None) == 0
+
+
+def test_the_reciprocal_that_places_pieces_is_exact():
+    """Rows of up to 2^16 pieces, counts up to pieces + 255: floor(at * ceil(2^32 / pieces) / 2^32) errs first at a multiple less one."""
+    pieces = torch.arange(2, 65537, dtype=torch.int64)
+    magic = (2 ** 32 + pieces - 1) // pieces
+    for k in range(1, 130):
+        at = k * pieces - 1
+        ok = at > pieces + 254
+        assert bool((ok | ((at * magic) >> 32 == at // pieces)).all())
