@@ -226,7 +226,9 @@ class CrossLayerTranscoder(BaseTranscoder):
     def quantise_encoder(self, fmt: str = "mxfp4") -> None:
         """Compute pre-activations from 4-bit weights and inputs from here on (inference: forward, activations, evaluation, theta
         estimation).  The parameters and checkpoints stay as they are, and what is written to them shows in the next forward;
-        ``dequantise_encoder()`` goes back.  Selection and decode are the same; training entry points raise meanwhile."""
+        ``dequantise_encoder()`` goes back.  Selection and decode are the same; training entry points raise meanwhile.  Captured
+        forwards use the 4-bit copy and are replayed only while it is there; forwards on several streams at once need the caller's
+        ordering, since each looks whether the copy is up to date."""
         self._sync_device()
         self.encoder_module.quantise(fmt)
 

@@ -1261,7 +1261,7 @@ extern "C" int clt_mx_encode(const void *x, const uint8_t *x_scales, const void 
   if (T < 0 || d <= 0 || F <= 0 || L <= 0) return CLT_ERR_ARG;
   if (T == 0) return CLT_OK;
   if (!x || !w_codes || !w_scales || !pre || pre_row_stride < F || pre_layer_stride < 0 || (!x_scales && x_layer_stride < 0)) return CLT_ERR_ARG;
-  if (d > MX_MAX_WIDTH || T > (1 << 20) || F > (1 << 30) || L > 32767) return CLT_ERR_RANGE;
+  if (d > MX_MAX_WIDTH || T > 16 * 65535 || F > (1 << 30) || L > 32767) return CLT_ERR_RANGE;
   if ((x_scales && !clt_aligned16(x)) || !clt_aligned16(w_codes)) return CLT_ERR_ALIGN;
   const int64_t e = clt_elem_bytes(dtype);
   const MxPlan p = mx_plan(T, d, F, L, x_scales != nullptr,

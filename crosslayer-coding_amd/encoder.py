@@ -105,13 +105,15 @@ class Encoder(nn.Module):
         L, F, d = w.shape
         weights = [own_parameter(enc, "weight") for enc in self.encoders._modules.values()]
         keys = tuple((p.data_ptr(), p._version) for p in weights)
+        capturing = torch.cuda.is_current_stream_capturing()
         if self._mx is None or self._mx.device != w.device or self._mx_keys != keys:
             out = self._mx if self._mx is not None and self._mx.device == w.device and self._mx.shape == w.shape else None
             with torch.no_grad():
                 self._mx = mx.quantise(w.detach(), self._mx_fmt, out=out)
-            self._mx_keys = keys
+            # a capture only records: its replays quantise, and the next eager call does so again
+            self._mx_keys = None if capturing else keys
             self._mx_state = None
-        if self.watch_parameter_data:
+        if self.watch_parameter_data and not (capturing and self._mx_state is None):
             fresh = self._mx_state is None
             if fresh:
                 self._mx_state = (torch.zeros(16 * L, dtype=torch.int64, device=w.device), torch.zeros(L, dtype=torch.int32, device=w.device))

@@ -915,7 +915,7 @@ int clt_feed_gather(const void *src, int src_dtype, int64_t src_rows, int64_t sr
  *   [L][T][d] values of dtype, layers x_layer_stride apart, which the call quantises, when x_scales is NULL; else its
  *   codes and scales [L][T].  pre rows are pre_row_stride >= F elements apart, layers pre_layer_stride.
  *   What clt_encode computes from 16- or 32-bit operands (clt/models/parallel.py:286).  workspace: 16-byte aligned,
- *   clt_mx_encode_workspace_bytes (may be 0 when x comes quantised).  T up to 2^20, F up to 2^30, L up to 32767.
+ *   clt_mx_encode_workspace_bytes (may be 0 when x comes quantised).  T up to 16 * 65535, F up to 2^30, L up to 32767.
  */
 #define CLT_MXFP4 0
 #define CLT_MXFP8 1

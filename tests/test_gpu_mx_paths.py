@@ -211,6 +211,35 @@ def test_captured_forward_of_a_quantised_model(dev, T):
                 assert torch.equal(got[l], want[l]), (trial, l)
 
 
+def test_forward_captured_right_after_the_weights_were_written(dev):
+    """Nothing that a capture recorded has run when the next eager forward comes."""
+    model, inputs, x = _model(dev, T=40)
+    model.quantise_encoder()
+    s = torch.cuda.Stream()
+    with torch.no_grad():
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            for _ in range(2):
+                model(inputs)
+        torch.cuda.current_stream().wait_stream(s)
+        weight = model.encoder_module.encoders[1].weight
+        weight.mul_(-0.5)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = model(inputs)
+        eager = {l: v.clone() for l, v in model(inputs).items()}
+        pre, _ = model._encode_all_layers(inputs)
+        want, tol = _with_values(model, x)
+        for l in inputs:
+            assert bool(((pre[l].cpu().double() - want[l]).abs() <= tol[l]).all())
+        for _ in range(3):
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(out[l], eager[l]) for l in eager)
+            again = model(inputs)
+            assert all(torch.equal(again[l], eager[l]) for l in eager)
+
+
 def test_a_cache_feeds_a_quantised_model(dev):
     """A harvest written to a quantised chunk, a batch drawn from it, and that batch through the model."""
     model, inputs, x = _model(dev, T=64)
