@@ -81,7 +81,8 @@ def _check_values(t: torch.Tensor, what: str) -> None:
 
 def _rows_2d(t: torch.Tensor) -> torch.Tensor:
     """[rows, d] with neighbouring elements next to each other, without a copy where the strides allow it."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
@@ -103,6 +104,13 @@ class MXTensor:
         if codes.data_ptr() % 16 != 0:
             raise ValueError("codes must begin at a multiple of 16 bytes")
         self.codes, self.scales, self.fmt, self.width = codes, scales, fmt, int(width)
+
+    @classmethod
+    def _made(cls, codes: torch.Tensor, scales: torch.Tensor, fmt: str, width: int) -> "MXTensor":
+        """Of tensors that were just allocated as `row_layout` says: nothing to check."""
+        held = cls.__new__(cls)
+        held.codes, held.scales, held.fmt, held.width = codes, scales, fmt, width
+        return held
 
     @property
     def shape(self) -> torch.Size:
@@ -146,8 +154,8 @@ def quantise(x: torch.Tensor, fmt: str = "mxfp4", out: Optional[MXTensor] = None
     _check_values(x, "quantise")
     if out is None:
         lead = x.shape[:-1]
-        out = MXTensor(torch.empty((*lead, pitch), dtype=torch.uint8, device=x.device),
-                       torch.empty((*lead, blocks), dtype=torch.uint8, device=x.device), fmt, x.shape[-1])
+        out = MXTensor._made(torch.empty((*lead, pitch), dtype=torch.uint8, device=x.device),
+                             torch.empty((*lead, blocks), dtype=torch.uint8, device=x.device), fmt, x.shape[-1])
     elif out.fmt != fmt or out.shape != x.shape or out.device != x.device:
         raise ValueError(f"out is {out.fmt} {tuple(out.shape)} on {out.device}, wanted {fmt} {tuple(x.shape)} on {x.device}")
     if x.numel() == 0:
@@ -362,13 +370,14 @@ class MXActivationCache:
         if out is None:
             if out_row != 0:
                 raise ValueError("out_row without out")
-            out = (torch.empty((L, n, d), dtype=dtype, device=self.device), torch.empty((L, n, d), dtype=dtype, device=self.device))
-        T = out[0].shape[1] if out[0].dim() == 3 else -1
-        for t in out:
-            if t.shape != (L, T, d) or t.dtype != dtype or t.device != self.device or not t.is_contiguous():
-                raise ValueError(f"out must be two contiguous {dtype} tensors [{L}, T, {d}] on {self.device}")
-        if out_row < 0 or out_row + n > T:
-            raise ValueError(f"rows {out_row} .. {out_row + n} are not in an output of {T} rows")
+            out, T = (torch.empty((L, n, d), dtype=dtype, device=self.device), torch.empty((L, n, d), dtype=dtype, device=self.device)), n
+        else:
+            T = out[0].shape[1] if out[0].dim() == 3 else -1
+            for t in out:
+                if t.shape != (L, T, d) or t.dtype != dtype or t.device != self.device or not t.is_contiguous():
+                    raise ValueError(f"out must be two contiguous {dtype} tensors [{L}, T, {d}] on {self.device}")
+            if out_row < 0 or out_row + n > T:
+                raise ValueError(f"rows {out_row} .. {out_row + n} are not in an output of {T} rows")
         held = (None,) * 4
         if normalization == "mean_std":
             if tables is None or len(tables) != 4 or any((tables[i] is None) != (tables[i + 1] is None) for i in (0, 2)):
@@ -376,14 +385,14 @@ class MXActivationCache:
             for t in tables:
                 if t is not None and (t.shape != (L, d) or t.dtype != torch.float32 or t.device != self.device or not t.is_contiguous()):
                     raise ValueError(f"the tables must be contiguous float32 [{L}, {d}] on {self.device}")
-            held = tuple(tables)
+            held = tuple(nat.ptr(t) for t in tables)
         if n == 0:
             return out[0], out[1]
         with _On(self.device):
             code = nat.load().clt_mx_cache_read(
                 nat.ptr(self.codes), nat.ptr(self.scales), self.rows, FORMATS[self.fmt], nat.ptr(index),
                 0 if index is None else 8 * index.element_size(), first, n, d, L, _NORM_MODES[normalization],
-                *(nat.ptr(t) for t in held), math.sqrt(d) if normalization == "sqrt_d_model" else 1.0, nat.ptr(out[0]), nat.ptr(out[1]),
+                *held, math.sqrt(d) if normalization == "sqrt_d_model" else 1.0, nat.ptr(out[0]), nat.ptr(out[1]),
                 out_row, T, nat.dtype_code(dtype), nat.current_stream(self.device))
         nat.check(code, "clt_mx_cache_read")
         return out[0], out[1]
