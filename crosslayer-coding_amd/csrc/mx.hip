@@ -112,8 +112,8 @@ __device__ __forceinline__ int64_t mx_row(const MxRows &r, int64_t j) {
 // A thread goes on to the same piece of `rows_apart` rows further on, so that several loads are under way and what belongs to
 // the column is fetched once.
 struct MxPiece { int64_t j; uint32_t p; };
-__device__ __forceinline__ MxPiece mx_piece(uint32_t pieces, uint32_t magic) {
-  const uint64_t base = (uint64_t)blockIdx.x * MX_THREADS;
+__device__ __forceinline__ MxPiece mx_piece(uint32_t group, uint32_t pieces, uint32_t magic) {
+  const uint64_t base = (uint64_t)group * MX_THREADS;
   const uint64_t row0 = base / pieces;
   const uint32_t at = (uint32_t)(base - row0 * pieces) + threadIdx.x;
   const uint32_t dj = pieces == 1u ? at : __umulhi(at, magic);
@@ -160,33 +160,44 @@ template <int FMT> __device__ __forceinline__ uint32_t mx_scale16(float (&v)[16]
 //
 // Bound by memory: 12 x 24576 rows of 768 bf16 to mxfp4 106 us (573 MB, 5.4 TB/s; past the caches 140 us); 12 layers of 4096 x 768 bf16,
 // inputs and targets, into mxfp8 49 us from memory, 28 us where the batch is still in the memory-side cache.
-template <typename T, int FMT, bool VEC>
-__global__ __launch_bounds__(MX_THREADS) void k_mx_write(const T *__restrict__ src0, const T *__restrict__ src1, int64_t layer_stride,
-                                                         int64_t row_stride, int kinds, int64_t n, int64_t d, uint32_t blocks,
-                                                         uint32_t magic, MxRows rows, uint8_t *__restrict__ codes,
-                                                         uint8_t *__restrict__ scales, int tiled) {
-  const MxPiece at = mx_piece(blocks * 2u, magic);
-  if (at.j >= n) return;                               // whole pairs: a row has whole blocks
+struct MxWrite {
+  const void *src0, *src1;
+  int64_t layer_stride, row_stride, n, d;
+  int kinds;
+  uint32_t blocks, magic;
+  MxRows rows;
+  uint8_t *codes, *scales;
+};
+template <typename T, int FMT, bool VEC, bool TILED>
+__device__ __forceinline__ void mx_write_piece(const MxWrite &a, uint32_t group) {
+  const int kinds = a.kinds;
+  const uint32_t blocks = a.blocks;
+  const MxRows &rows = a.rows;
+  const MxPiece at = mx_piece(group, blocks * 2u, a.magic);
+  if (at.j >= a.n) return;                               // whole pairs: a row has whole blocks
   const int64_t l = blockIdx.y / (uint32_t)kinds;
   const int kind = (int)(blockIdx.y - (uint32_t)l * (uint32_t)kinds);
   const int64_t c = (int64_t)at.p * 16;
-  const T *sp = (kind ? src1 : src0) + l * layer_stride + at.j * row_stride + c;
+  const T *sp = (const T *)(kind ? a.src1 : a.src0) + l * a.layer_stride + at.j * a.row_stride + c;
   float v[16];
-  mx_load8<T, VEC>(sp, d - c, v);
-  mx_load8<T, VEC>(sp + 8, d - c - 8, v + 8);
+  mx_load8<T, VEC>(sp, a.d - c, v);
+  mx_load8<T, VEC>(sp + 8, a.d - c - 8, v + 8);
   const int64_t r = mx_row(rows, at.j);
   const uint32_t s = mx_scale16<FMT>(v);
   if (r < 0 || r >= rows.rows) return;                 // a row outside the store is not written
   if (rows.owner && rows.owner[r] != (int32_t)at.j) return;
   const uint64_t row = ((uint64_t)l * (uint32_t)kinds + (uint32_t)kind) * (uint64_t)rows.rows + (uint64_t)r;
-  const uint2 a = mx_encode8<FMT>(*reinterpret_cast<float (*)[8]>(v)), b = mx_encode8<FMT>(*reinterpret_cast<float (*)[8]>(v + 8));
-  if constexpr (FMT == CLT_MXFP4) *reinterpret_cast<uint2 *>(codes + row * blocks * 16u + at.p * 8u) = make_uint2(a.x, b.x);
-  else *reinterpret_cast<uint4 *>(codes + row * blocks * 32u + at.p * 16u) = make_uint4(a.x, a.y, b.x, b.y);
+  const uint2 lo = mx_encode8<FMT>(*reinterpret_cast<float (*)[8]>(v)), hi = mx_encode8<FMT>(*reinterpret_cast<float (*)[8]>(v + 8));
+  if constexpr (FMT == CLT_MXFP4) *reinterpret_cast<uint2 *>(a.codes + row * blocks * 16u + at.p * 8u) = make_uint2(lo.x, hi.x);
+  else *reinterpret_cast<uint4 *>(a.codes + row * blocks * 32u + at.p * 16u) = make_uint4(lo.x, lo.y, hi.x, hi.y);
   if ((at.p & 1u) == 0u) {
     const uint32_t blk = at.p >> 1;
-    if (!tiled) scales[row * blocks + blk] = (uint8_t)s;
-    else scales[row / MX_BM * MX_BM * blocks + (blk / 8) * (MX_BM * 8) + mx_scale_place((uint32_t)(row % MX_BM), blk % 8, MX_MG)] = (uint8_t)s;
+    if constexpr (!TILED) a.scales[row * blocks + blk] = (uint8_t)s;
+    else a.scales[row / MX_BM * MX_BM * blocks + (blk / 8) * (MX_BM * 8) + mx_scale_place((uint32_t)(row % MX_BM), blk % 8, MX_MG)] = (uint8_t)s;
   }
+}
+template <typename T, int FMT, bool VEC> __global__ __launch_bounds__(MX_THREADS) void k_mx_write(MxWrite a) {
+  mx_write_piece<T, FMT, VEC, false>(a, blockIdx.x);
 }
 
 // ---- weights that may have been written -------------------------------------------------------------------------------
@@ -313,7 +324,7 @@ __global__ __launch_bounds__(MX_THREADS) void k_mx_read(const uint8_t *__restric
                                                         uint32_t magic, int kinds, MxNorm nm, OutT *__restrict__ out0,
                                                         OutT *__restrict__ out1, int64_t out_layer_stride, int64_t out_row_stride) {
   constexpr int E = VEC && sizeof(OutT) == 4 ? 4 : 8;
-  const MxPiece at = mx_piece(pieces, magic);
+  const MxPiece at = mx_piece(blockIdx.x, pieces, magic);
   if (at.j >= rows_apart) return;
   const int64_t l = blockIdx.y / (uint32_t)kinds;
   const int kind = (int)(blockIdx.y - (uint32_t)l * (uint32_t)kinds);
@@ -928,31 +939,53 @@ __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 }
 
 // What a tile takes beside its codes: the scales of its 256 rows in the lanes' order, zeros where there is no block or no row, and the
-// biases in float32.  grid: x = tiles, y = layers; a thread writes two words of every stage.
-template <typename T, int GROUPS>
-__global__ __launch_bounds__(256) void k_mx_tile_side(const uint8_t *__restrict__ scales, uint8_t *__restrict__ out, const T *__restrict__ bias,
-                                                      float *__restrict__ bias_out, int rows, int blocks, int stages, int64_t bs) {
-  const int64_t l = blockIdx.y, tile = l * gridDim.x + blockIdx.x;
+// biases in float32.  A workgroup takes one stage of one tile: a thread fetches the eight scales of a row and puts out two words.
+struct MxSide {
+  const uint8_t *scales;
+  uint8_t *out;
+  const void *bias;
+  float *bias_out;
+  int rows, blocks, stages;
+  int64_t bias_stride;
+};
+template <typename T, int GROUPS> __device__ __forceinline__ void mx_tile_side(const MxSide &a, int x, int tile0, int64_t l) {
+  __shared__ uint2 held[256];
+  const int stage = x % a.stages, t = x / a.stages;
+  const int64_t tile = l * tile0 + t;
   // feature tiles: the last one is moved back inside the matrix
-  const int r0 = GROUPS == 8 ? min((int)blockIdx.x * 256, rows - 256) : (int)blockIdx.x * 256;
-  for (int s = 0; s < stages; ++s) {
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int at = half * 256 + threadIdx.x, lane = at % 64, i0 = at / 64 % (GROUPS / 2) * 2, w = at / (32 * GROUPS);
-      const int b = s * TBLOCKS + (lane >> 4);
-      uint32_t v = 0;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = r0 + (w * GROUPS + i0 + i) * 16 + (lane & 15);
-        if (r < rows) {
-          const uint8_t *p = scales + (l * rows + r) * blocks + b;
-          v |= ((b < blocks ? (uint32_t)p[0] : 0u) | (b + 4 < blocks ? (uint32_t)p[4] << 8 : 0u)) << (i * 16);
-        }
-      }
-      *reinterpret_cast<uint32_t *>(out + (tile * stages + s) * 2048 + at * 4) = v;
+  const int r0 = GROUPS == 8 ? min(t * 256, a.rows - 256) : t * 256, r = r0 + (int)threadIdx.x, b0 = stage * TBLOCKS;
+  uint2 v = make_uint2(0u, 0u);
+  if (r < a.rows) {
+    const uint8_t *p = a.scales + (l * a.rows + r) * a.blocks + b0;
+    if (b0 + TBLOCKS <= a.blocks) __builtin_memcpy(&v, p, 8);
+    else {
+      for (int b = 0; b0 + b < a.blocks; ++b) (b < 4 ? v.x : v.y) |= (uint32_t)p[b] << (b % 4 * 8);
     }
   }
-  if (bias_out) bias_out[tile * 256 + threadIdx.x] = bias ? Elem<T>::to_f32(bias[l * bs + r0 + threadIdx.x]) : 0.0f;
+  held[threadIdx.x] = v;
+  __syncthreads();
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int at = half * 256 + threadIdx.x, lane = at % 64, i0 = at / 64 % (GROUPS / 2) * 2, w = at / (32 * GROUPS), shift = (lane >> 4) * 8;
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint2 h = held[(w * GROUPS + i0 + i) * 16 + (lane & 15)];
+      word |= ((h.x >> shift & 255u) | (h.y >> shift & 255u) << 8) << (i * 16);
+    }
+    *reinterpret_cast<uint32_t *>(a.out + (tile * a.stages + stage) * 2048 + at * 4) = word;
+  }
+  if (a.bias_out && stage == 0) a.bias_out[tile * 256 + threadIdx.x] = a.bias ? Elem<T>::to_f32(((const T *)a.bias)[l * a.bias_stride + r]) : 0.0f;
+}
+template <typename T, int GROUPS> __global__ __launch_bounds__(256) void k_mx_tile_side(MxSide a) {
+  mx_tile_side<T, GROUPS>(a, blockIdx.x, gridDim.x / a.stages, blockIdx.y);
+}
+// The same for the weights beside the quantisation of x, neither of which waits for the other: 8.2 us for 77 tokens of 12 x 24576 x 768,
+// 150 us for 8192 of 16 x 16384 x 2048 (0.72 GB); as two launches, a thread going through a tile's stages, 5.0 + 7.6 and 136 + 38 us.
+template <typename T, bool VEC> __global__ __launch_bounds__(256) void k_mx_tile_inputs(MxSide a, int tiles, MxWrite x) {
+  const int side = tiles * a.stages;
+  if ((int)blockIdx.x < side) mx_tile_side<T, 8>(a, blockIdx.x, tiles, blockIdx.y);
+  else mx_write_piece<T, CLT_MXFP4, VEC, true>(x, blockIdx.x - side);
 }
 
 // Rows of codes at another pitch, `to` blocks of 16 bytes instead of `from`, filled up with zeros; the rows of a layer `room` rows
@@ -978,37 +1011,36 @@ constexpr int MX_U = 2;
 constexpr int64_t MX_MANY = 4 * 1024 * 64;
 uint32_t mx_magic(uint32_t pieces) { return (uint32_t)((0x100000000ull + pieces - 1) / pieces); }
 
+template <typename T>
+bool mx_write_vec(const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t d) {
+  return d % 8 == 0 && clt_aligned16(src0) && clt_aligned16(src1) && row_stride * (int64_t)sizeof(T) % 16 == 0 && layer_stride * (int64_t)sizeof(T) % 16 == 0;
+}
+
 template <typename T, int FMT>
 int launch_mx_write(const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t L, int kinds, int64_t n, int64_t d,
-                    uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, hipStream_t s) {
-  const uint32_t pieces = blocks * 2;
-  const int64_t groups = clt_ceil_div(n * (int64_t)pieces, MX_THREADS);
+                    uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, hipStream_t s) {
+  const int64_t groups = clt_ceil_div(n * (int64_t)(blocks * 2), MX_THREADS);
   if (groups > 2147483647LL) return CLT_ERR_RANGE;
-  const bool vec = d % 8 == 0 && clt_aligned16(src0) && (kinds == 1 || clt_aligned16(src1)) && (row_stride * (int64_t)sizeof(T)) % 16 == 0 &&
-                   (layer_stride * (int64_t)sizeof(T)) % 16 == 0;
   const dim3 grid((unsigned)groups, (unsigned)(L * kinds));
-#define CLT_MXW(VEC)                                                                                                               \
-  k_mx_write<T, FMT, VEC><<<grid, MX_THREADS, 0, s>>>((const T *)src0, (const T *)src1, layer_stride, row_stride, kinds, n, d, blocks, \
-                                                      mx_magic(pieces), rows, (uint8_t *)codes, scales, tiled)
-  if (vec) CLT_MXW(true);
-  else CLT_MXW(false);
-#undef CLT_MXW
+  const MxWrite a{src0, src1, layer_stride, row_stride, n, d, kinds, blocks, mx_magic(blocks * 2), rows, (uint8_t *)codes, scales};
+  if (mx_write_vec<T>(src0, src1, layer_stride, row_stride, d)) k_mx_write<T, FMT, true><<<grid, MX_THREADS, 0, s>>>(a);
+  else k_mx_write<T, FMT, false><<<grid, MX_THREADS, 0, s>>>(a);
   return clt_check_launch();
 }
 
 template <typename T>
 int mx_write_as(int fmt, const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t L, int kinds, int64_t n,
-                int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, hipStream_t s) {
-  if (fmt == CLT_MXFP4) return launch_mx_write<T, CLT_MXFP4>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
-  if (fmt == CLT_MXFP8) return launch_mx_write<T, CLT_MXFP8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
-  return launch_mx_write<T, CLT_MXINT8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
+                int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, hipStream_t s) {
+  if (fmt == CLT_MXFP4) return launch_mx_write<T, CLT_MXFP4>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
+  if (fmt == CLT_MXFP8) return launch_mx_write<T, CLT_MXFP8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
+  return launch_mx_write<T, CLT_MXINT8>(src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
 }
 
 int mx_write(int dtype, int fmt, const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t L, int kinds,
-             int64_t n, int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, int tiled, hipStream_t s) {
-  if (dtype == CLT_BF16) return mx_write_as<bf16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
-  if (dtype == CLT_F16) return mx_write_as<f16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
-  return mx_write_as<float>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, tiled, s);
+             int64_t n, int64_t d, uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, hipStream_t s) {
+  if (dtype == CLT_BF16) return mx_write_as<bf16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
+  if (dtype == CLT_F16) return mx_write_as<f16_t>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
+  return mx_write_as<float>(fmt, src0, src1, layer_stride, row_stride, L, kinds, n, d, blocks, rows, codes, scales, s);
 }
 
 template <typename OutT, int FMT>
@@ -1111,15 +1143,22 @@ int mx_grid(int64_t tiles) {
 }
 
 template <typename OutT>
-int launch_mx_project(const MxPlan &p, const void *xc, int64_t x_layer, bool vec, const uint8_t *xs, const uint8_t *wc, const uint8_t *wsc, const void *bias,
+int launch_mx_project(const MxPlan &p, const void *x, const void *xc, int64_t x_layer, bool vec, const uint8_t *xs, const uint8_t *wc, const uint8_t *wsc, const void *bias,
                       uint8_t *ws, void *pre, int64_t T, int64_t d, int64_t F, int64_t L, int64_t bs, int64_t ps, int64_t pre_row, hipStream_t s) {
   if (p.tiles) {
     const int64_t total = p.tm * p.tn * L;
-    if (total > 1073741824LL) return CLT_ERR_RANGE;
+    if (total > 1073741824LL || p.tn * p.stages > 1073741824LL || p.tm * p.stages > 1073741824LL) return CLT_ERR_RANGE;
     const int grid = mx_grid(total);
     if (grid <= 0) return CLT_ERR_LAUNCH;
-    k_mx_tile_side<OutT, 8><<<dim3((unsigned)p.tn, (unsigned)L), 256, 0, s>>>(wsc, ws + p.ws, (const OutT *)bias, (float *)(ws + p.bias), (int)F,
-                                                                              (int)p.blocks, (int)p.stages, bs);
+    const MxSide side{wsc, ws + p.ws, bias, (float *)(ws + p.bias), (int)F, (int)p.blocks, (int)p.stages, bs};
+    if (x) {                                               // values, to be quantised into the workspace
+      const uint32_t pieces = (uint32_t)p.padded * 2;
+      const int64_t groups = p.tn * p.stages + clt_ceil_div(T * pieces, MX_THREADS);
+      const dim3 grid((unsigned)groups, (unsigned)L);
+      const MxWrite w{x, nullptr, x_layer, d, T, d, 1, (uint32_t)p.padded, mx_magic(pieces), {nullptr, 0, 0, p.xrows, nullptr}, ws + p.xc, ws + p.xs};
+      if (vec) k_mx_tile_inputs<OutT, true><<<grid, 256, 0, s>>>(side, (int)p.tn, w);
+      else k_mx_tile_inputs<OutT, false><<<grid, 256, 0, s>>>(side, (int)p.tn, w);
+    } else k_mx_tile_side<OutT, 8><<<dim3((unsigned)(p.tn * p.stages), (unsigned)L), 256, 0, s>>>(side);
     TileArgs a{(const uint8_t *)xc, wc, xs, ws + p.ws, (const float *)(ws + p.bias), (int)T, (int)p.xrows, (int)F, (int)p.tm, (int)p.tn, (int)total,
                (int)clt_ceil_div(total, 8), (int)p.stages, (int)p.padded * 16, (int)p.blocks * 16, ps, pre_row,
                mx_div((uint32_t)(p.tm * p.tn)), mx_div((uint32_t)(8 * p.tm)), mx_div((uint32_t)(p.tn % 8 ? p.tn % 8 : 8)), mx_div((uint32_t)p.stages)};
@@ -1177,7 +1216,7 @@ extern "C" int clt_mx_quantise(const void *src, int64_t n, int64_t d, int64_t ro
   if (!src || !codes || !scales || (n > 1 && row_stride < d)) return CLT_ERR_ARG;
   if (!clt_aligned16(codes)) return CLT_ERR_ALIGN;
   const MxRows rows{nullptr, 0, 0, n, nullptr};
-  return mx_write(dtype, fmt, src, nullptr, 0, row_stride, 1, 1, n, d, (uint32_t)clt_ceil_div(d, 32), rows, codes, scales, 0, (hipStream_t)stream);
+  return mx_write(dtype, fmt, src, nullptr, 0, row_stride, 1, 1, n, d, (uint32_t)clt_ceil_div(d, 32), rows, codes, scales, (hipStream_t)stream);
 }
 
 extern "C" int clt_mx_refresh(const void *src, int64_t L, int64_t n, int64_t d, int64_t layer_stride, int dtype, void *codes, uint8_t *scales,
@@ -1223,7 +1262,7 @@ extern "C" int clt_mx_cache_write(const void *x, const void *tgt, int64_t layer_
     k_mx_claim<<<nb, 256, 0, s>>>(r, n, owner, 0);
     k_mx_claim<<<nb, 256, 0, s>>>(r, n, owner, 1);
   }
-  return mx_write(dtype, fmt, x, tgt, layer_stride, row_stride, L, 2, n, d, (uint32_t)clt_ceil_div(d, 32), r, codes, scales, 0, s);
+  return mx_write(dtype, fmt, x, tgt, layer_stride, row_stride, L, 2, n, d, (uint32_t)clt_ceil_div(d, 32), r, codes, scales, s);
 }
 
 extern "C" int clt_mx_cache_read(const void *codes, const uint8_t *scales, int64_t rows, int fmt, const void *row_index, int index_bits,
@@ -1276,22 +1315,24 @@ extern "C" int clt_mx_encode(const void *x, const uint8_t *x_scales, const void 
   const bool vec = d % 8 == 0 && clt_aligned16(x) && x_layer_stride * e % 16 == 0 && d * e % 16 == 0;
   int rc = CLT_OK;
   if (!x_scales && p.own_x) {
-    const MxRows rows{nullptr, 0, 0, p.xrows, nullptr};
-    rc = mx_write(dtype, CLT_MXFP4, x, nullptr, x_layer_stride, d, L, 1, T, d, (uint32_t)p.padded, rows, ws + p.xc, ws + p.xs, p.tiles, s);
     xc = ws + p.xc;
     xs = ws + p.xs;
+    if (!p.tiles) {
+      const MxRows rows{nullptr, 0, 0, p.xrows, nullptr};
+      rc = mx_write(dtype, CLT_MXFP4, x, nullptr, x_layer_stride, d, L, 1, T, d, (uint32_t)p.padded, rows, ws + p.xc, ws + p.xs, s);
+    }
   } else if (p.tiles) {
     if (p.own_x) {
       rc = launch_mx_widen(x, ws + p.xc, L, T, p.xrows, p.blocks, p.padded, s);
       xc = ws + p.xc;
     }
-    k_mx_tile_side<float, MX_MG><<<dim3((unsigned)p.tm, (unsigned)L), 256, 0, s>>>(x_scales, ws + p.xs, nullptr, nullptr, (int)T, (int)p.blocks,
-                                                                                   (int)p.stages, 0);
+    const MxSide side{x_scales, ws + p.xs, nullptr, nullptr, (int)T, (int)p.blocks, (int)p.stages, 0};
+    k_mx_tile_side<float, MX_MG><<<dim3((unsigned)(p.tm * p.stages), (unsigned)L), 256, 0, s>>>(side);
     xs = ws + p.xs;
   }
   if (rc != CLT_OK) return rc;
 #define CLT_MXE(T_) \
-  launch_mx_project<T_>(p, xc, x_layer_stride, vec, xs, wc, w_scales, bias, ws, pre, T, d, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s)
+  launch_mx_project<T_>(p, x_scales ? nullptr : x, xc, x_layer_stride, vec, xs, wc, w_scales, bias, ws, pre, T, d, F, L, b_layer_stride, pre_layer_stride, pre_row_stride, s)
   if (dtype == CLT_BF16) return CLT_MXE(bf16_t);
   if (dtype == CLT_F16) return CLT_MXE(f16_t);
   return CLT_MXE(float);
