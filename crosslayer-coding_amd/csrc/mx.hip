@@ -202,7 +202,8 @@ template <typename T, int FMT, bool VEC> __global__ __launch_bounds__(MX_THREADS
 
 // ---- weights that may have been written -------------------------------------------------------------------------------
 // Whether rows [L][n][d] still are what their fingerprint says: 64 bytes of every row, at places that go round, so that every row
-// and, from d / 32 rows on (16 bits), every column is looked at.  A layer's sums are of whole numbers, in any order; its last workgroup compares and stores.
+// and, from d / 32 rows on (16 bits), every column is looked at.  A layer's sums are of whole numbers, in any order; its last
+// workgroup compares and stores.
 // state: [L][16], a 128-byte line per layer: sum, workgroups that have arrived, fingerprint.
 //
 // 12 x 24576 rows of 768 bf16: 19 MB in 64-byte pieces, 21 us, of a layer's 64 workgroups with six loads in flight a lane; bound by
@@ -586,8 +587,8 @@ __global__ __launch_bounds__(256, 2) void k_mx_project_few(FewArgs a, const OutT
 // A stage is 256 elements of K: 128 bytes of codes per row - whole cache lines - brought straight into LDS, chunk c of row r at
 // chunk position c ^ ((r >> 1) & 7): a fragment read's lanes are served in sixteens that take half their rows from one quarter of
 // the wavefront and half from the next, and these places lie in all banks for the blocks lq and lq + 4 that a lane multiplies (lq =
-// lane / 16; 2 lq and 2 lq + 1 met in pairs, which cost half of LDS's cycles).  Scales come as the lanes take them (mx_scale_place): one word holds those of
-// two row groups and both blocks.
+// lane / 16; 2 lq and 2 lq + 1 met in pairs, which cost half of LDS's cycles).  Scales come as the lanes take them
+// (mx_scale_place): one word holds those of two row groups and both blocks.
 //
 // A stage is four quarters of 4 MG products: all tokens of the wavefront x 32 of its features.  The x fragments stay in
 // registers for the stage, each being replaced by the next stage's behind its last use; the W fragments of the next quarter are
@@ -603,9 +604,11 @@ __global__ __launch_bounds__(256, 2) void k_mx_project_few(FewArgs a, const OutT
 // so the waits for loads allow for the stores sent behind them.
 //
 // Measured on 12 x 4096 x 768 x 24576, bf16 out (2.42 GB: 405 - 450 us for a kernel that does nothing but store these tiles):
-// 647 us, without loads 558, without stores 504, without both 427 (of which the products alone would be 281 at the 6.6 PFLOP/s that
-// the power limit leaves them on random operands).  On 16 x 8192 x 2048 x 16384: 2330 us (3780 TFLOP/s); 4 products of 8192^3:
-// 1010 - 1030 us (4340).  What did not help: groups of 4, 16 or 32 feature tiles in the order of the tiles (650 - 660 us).
+// 600 us, without loads 531, without stores 472, without both 406 (of which the products alone would be 281 at the 6.6 PFLOP/s that
+// the power limit leaves them on random operands).  On 16 x 8192 x 2048 x 16384: 2160 - 2230 us (4000 TFLOP/s); 4 products of
+// 8192^3: 960 us (4580).  Beside the stores it is bound by the LDS: per 128 of K its wavefronts read 96 KB from it and 32 KB are put
+// in, 1024 of its cycles at 128 bytes each, as many as the products themselves take at their full rate.  What did not help: groups
+// of 4, 16 or 32 feature tiles in the order of the tiles (3 - 5 us slower).
 constexpr int TW = 8;                         // wavefronts
 constexpr int TROW = 128;                     // bytes of codes per row and stage
 // Of a buffer store, taken where the rows of the result begin with a cache line (LINES): its parts are whole lines, and past the caches
@@ -1085,8 +1088,8 @@ int mx_read(int dtype, int fmt, const void *codes, const uint8_t *scales, const 
 // How a shape is computed.  Up to 64 tokens, as long as their rows leave room in LDS for two workgroups per CU, by the kernel for few:
 // W is read once then.  Beyond by tiles, where there are whole feature tiles and rows of the result lie at whole words (buffer
 // stores); else by the kernel for few in groups of tokens.  12 layers, d 768, F 24576, bf16, kernel for few against tiles, us, x
-// quantised in the call: 26 against 46 at 1 token, 30 / 47 at 17, 34 / 47 at 33, 62 / 48 at 77, 78 / 50 at 128, 147 / 59 at 256;
-// 16 layers, d 2048, F 16384: 78 / 100 at 17, 94 / 104 at 64.
+// quantised in the call: 26 against 47 at 1 token, 30 / 45 at 17, 34 / 46 at 33, 40 / 46 at 64, 63 / 50 at 77, 75 / 50 at 128, 148 / 57
+// at 256; 16 layers, d 2048, F 16384: 78 / 97 at 17, 95 / 99 at 64.
 bool mx_tiles_fit(int64_t F, const void *pre, int64_t ps, int64_t pre_row, int64_t e) {
   return ((uintptr_t)pre & 3u) == 0 && ps * e % 4 == 0 && pre_row * e % 4 == 0 && F * e % 4 == 0 && pre_row * e <= (1 << 22);
 }
