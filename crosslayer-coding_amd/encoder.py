@@ -126,7 +126,9 @@ class Encoder(nn.Module):
         if self._mx_fmt is None:
             return engine.encode(x, w, b, out=out)
         q = self.quantised_weights()
-        if layers != list(range(self.config.num_layers)):
+        if layers == list(range(layers[0], layers[0] + len(layers))):
+            q = q.narrow(layers[0], len(layers))
+        else:
             q = q.index_select(torch.tensor(layers, device=w.device))
         with torch.no_grad():
             return mx.project(x, q, b.detach(), out=out, ws=ws)

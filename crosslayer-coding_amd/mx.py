@@ -128,6 +128,10 @@ class MXTensor:
         """The entries ``index`` of the first dimension, copied."""
         return MXTensor(self.codes.index_select(0, index), self.scales.index_select(0, index), self.fmt, self.width)
 
+    def narrow(self, first: int, n: int) -> "MXTensor":
+        """The entries first, ..., first + n - 1 of the first dimension, not copied."""
+        return MXTensor(self.codes.narrow(0, first, n), self.scales.narrow(0, first, n), self.fmt, self.width)
+
     def dequantise(self, dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The values the codes stand for (``out``: contiguous, of this shape)."""
         nat.require_device(self.codes, "MXTensor.dequantise")
@@ -234,6 +238,9 @@ def project(x: Union[torch.Tensor, MXTensor], w: MXTensor, b: Optional[torch.Ten
     given = isinstance(x, MXTensor)
     if not given:
         x = x.contiguous()
+        at, to, e = x.data_ptr(), out.data_ptr(), x.element_size()
+        if to < at + x.numel() * e and at < to + out.numel() * e:
+            raise ValueError("out lies in x: workgroups would read what others have written")
     T, F = shape[-2], shape[-1]
     L = shape[0] if len(shape) == 3 else 1
     lib = nat.load()

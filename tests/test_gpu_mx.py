@@ -448,3 +448,25 @@ def test_refresh_follows_writes_to_any_row_column_or_layer(dev, dtype, L, n, d):
             _check_codes(q, w.cpu(), "mxfp4")
             cca.mx.refresh(w, q, state, changed)
             assert not changed.any()
+
+
+def test_an_output_inside_the_input_is_refused(dev):
+    w = cca.mx.quantise(torch.randn(256, 256, device=dev))
+    buf = torch.randn(80, 256, device=dev)
+    before = buf.clone()
+    for a, b in ((0, 0), (0, 20), (20, 0)):
+        with pytest.raises(ValueError, match="out lies in x"):
+            cca.mx.project(buf[a:a + 40], w, out=buf[b:b + 40])
+    assert torch.equal(buf, before)
+    assert torch.equal(cca.mx.project(buf[:40], w, out=buf[40:]), cca.mx.project(before[:40], w))
+    strided = torch.randn(40, 512, device=dev)[:, ::2]
+    assert torch.equal(cca.mx.project(strided, w), cca.mx.project(strided.contiguous(), w))
+
+
+@pytest.mark.parametrize("first,n", [(0, 3), (1, 1), (2, 1), (1, 2)])
+def test_narrowed_weights_are_the_layers_themselves(dev, first, n):
+    q = cca.mx.quantise(torch.randn(3, 300, 100, device=dev))
+    x = torch.randn(n, 5, 100, device=dev)
+    part = q.narrow(first, n)
+    assert part.codes.data_ptr() == q.codes[first].data_ptr() and part.shape == (n, 300, 100)
+    assert torch.equal(cca.mx.project(x, part), cca.mx.project(x, q.index_select(torch.arange(first, first + n, device=dev))))
