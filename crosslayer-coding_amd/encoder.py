@@ -101,8 +101,13 @@ class Encoder(nn.Module):
         """The copy, true to the parameters: made anew where a parameter's storage or version counter changed, and by the
         device itself for layers whose data alone did (``weight.data.fill_(...)``: every row and column of a weight is looked
         at; ``watch_parameter_data`` = False leaves that out)."""
-        w, _ = self.stacked()
-        L, F, d = w.shape
+        self.stacked()
+        return self._quantised_slab()
+
+    def _quantised_slab(self, first: int = 0, n: Optional[int] = None) -> mx.MXTensor:
+        """`quantised_weights` of the slab as `stacked` has left it; n layers from ``first`` on (default: all) are looked at."""
+        w = self._w_slab
+        L = w.shape[0]
         weights = [own_parameter(enc, "weight") for enc in self.encoders._modules.values()]
         keys = tuple((p.data_ptr(), p._version) for p in weights)
         capturing = torch.cuda.is_current_stream_capturing()
@@ -114,22 +119,25 @@ class Encoder(nn.Module):
             self._mx_keys = None if capturing else keys
             self._mx_state = None
         if self.watch_parameter_data and not (capturing and self._mx_state is None):
-            fresh = self._mx_state is None
-            if fresh:
+            if self._mx_state is None:
                 self._mx_state = (torch.zeros(16 * L, dtype=torch.int64, device=w.device), torch.zeros(L, dtype=torch.int32, device=w.device))
-            mx.refresh(w.detach(), self._mx, *self._mx_state, store_only=fresh)
-        return self._mx
+                mx.refresh(w.detach(), self._mx, *self._mx_state, store_only=True)
+            else:
+                mx.refresh(w.detach(), self._mx, *self._mx_state, first=first, n=n)
+        return self._mx if n is None else self._mx.narrow(first, n)
 
     def project(self, layers: List[int], x: torch.Tensor, w: torch.Tensor, b: torch.Tensor, out: Optional[torch.Tensor] = None,
                 ws: Optional[engine.Workspace] = None) -> torch.Tensor:
         """Pre-activations of ``prepare_slab``'s (layers, x, w, b), from the 4-bit weights where there are some."""
         if self._mx_fmt is None:
             return engine.encode(x, w, b, out=out)
-        q = self.quantised_weights()
-        if layers == list(range(layers[0], layers[0] + len(layers))):
-            q = q.narrow(layers[0], len(layers))
+        first, n = layers[0], len(layers)
+        if n == self.config.num_layers:
+            q = self._quantised_slab()
+        elif layers == list(range(first, first + n)):
+            q = self._quantised_slab(first, n)
         else:
-            q = q.index_select(torch.tensor(layers, device=w.device))
+            q = self._quantised_slab().index_select(torch.tensor(layers, device=w.device))
         with torch.no_grad():
             return mx.project(x, q, b.detach(), out=out, ws=ws)
 

@@ -107,7 +107,7 @@ class MXTensor:
 
     @classmethod
     def _made(cls, codes: torch.Tensor, scales: torch.Tensor, fmt: str, width: int) -> "MXTensor":
-        """Of tensors that were just allocated as `row_layout` says: nothing to check."""
+        """Of tensors that are as `row_layout` says: nothing to check."""
         held = cls.__new__(cls)
         held.codes, held.scales, held.fmt, held.width = codes, scales, fmt, width
         return held
@@ -130,7 +130,7 @@ class MXTensor:
 
     def narrow(self, first: int, n: int) -> "MXTensor":
         """The entries first, ..., first + n - 1 of the first dimension, not copied."""
-        return MXTensor(self.codes.narrow(0, first, n), self.scales.narrow(0, first, n), self.fmt, self.width)
+        return MXTensor._made(self.codes.narrow(0, first, n), self.scales.narrow(0, first, n), self.fmt, self.width)
 
     def dequantise(self, dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The values the codes stand for (``out``: contiguous, of this shape)."""
@@ -174,25 +174,31 @@ def quantise(x: torch.Tensor, fmt: str = "mxfp4", out: Optional[MXTensor] = None
     return out
 
 
-def refresh(x: torch.Tensor, out: MXTensor, state: torch.Tensor, changed: torch.Tensor, store_only: bool = False) -> None:
-    """Bring the mxfp4 copy ``out`` of weights ``x`` [L, n, d] up to date where they were written since the last call, decided on the
+def refresh(x: torch.Tensor, out: MXTensor, state: torch.Tensor, changed: torch.Tensor, store_only: bool = False,
+            first: int = 0, n: Optional[int] = None) -> None:
+    """Bring the mxfp4 copy ``out`` of weights ``x`` [L, F, d] up to date where they were written since the last call, decided on the
     device: fingerprints of every layer (64 bytes of every row) in ``state`` (int64 [16 L], zeros before the first call) are
     compared, ``changed`` (int32 [L]) says which differ, and those layers are quantised anew.  ``store_only`` records the
-    fingerprints of weights that ``out`` was just made from."""
+    fingerprints of weights that ``out`` was just made from.  ``first``, ``n``: these layers alone (default: all)."""
     _check_values(x, "refresh")
     if x.dim() != 3 or out.fmt != "mxfp4" or out.shape != x.shape or out.device != x.device or x.stride(2) != 1 or x.stride(1) != x.shape[2]:
         raise ValueError(f"x {tuple(x.shape)} must be rows without gaps, out mxfp4 of its shape: got {out.fmt} {tuple(out.shape)}")
-    L = x.shape[0]
+    L, F, d = x.shape
     if state.dtype != torch.int64 or state.shape != (16 * L,) or changed.dtype != torch.int32 or changed.shape != (L,):
         raise ValueError(f"state must be int64 [{16 * L}], changed int32 [{L}]")
-    if state.device != x.device or changed.device != x.device:
-        raise ValueError(f"state and changed must be on {x.device}")
-    if x.numel() == 0:
+    if state.device != x.device or changed.device != x.device or not state.is_contiguous() or not changed.is_contiguous():
+        raise ValueError(f"state and changed must be contiguous and on {x.device}")
+    n = L - first if n is None else n
+    if first < 0 or n < 0 or first + n > L:
+        raise IndexError(f"layers {first} .. {first + n} are not in weights of {L} layers")
+    if n == 0 or F == 0:
         return
+    rows = first * F
     with _On(x.device):
-        code = nat.load().clt_mx_refresh(nat.ptr(x), L, x.shape[1], x.shape[2], x.stride(0), nat.dtype_code(x.dtype), nat.ptr(out.codes),
-                                         nat.ptr(out.scales), nat.ptr(state), nat.ptr(changed), 1 if store_only else 0,
-                                         nat.current_stream(x.device))
+        code = nat.load().clt_mx_refresh(
+            x.data_ptr() + first * x.stride(0) * x.element_size(), n, F, d, x.stride(0), nat.dtype_code(x.dtype),
+            out.codes.data_ptr() + rows * out.codes.shape[2], out.scales.data_ptr() + rows * out.scales.shape[2], state.data_ptr() + 128 * first,
+            changed.data_ptr() + 4 * first, 1 if store_only else 0, nat.current_stream(x.device))
     nat.check(code, "clt_mx_refresh")
 
 

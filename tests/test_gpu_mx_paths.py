@@ -156,6 +156,30 @@ def test_writes_to_the_weights_show(dev):
     check()
 
 
+def test_writes_show_in_single_layers_too(dev):
+    """A layer's own look at its weights leaves the others' for their next use."""
+    model, inputs, x = _model(dev, T=20)
+    model.quantise_encoder()
+
+    def check(*layers):
+        want, tol = _with_values(model, x)
+        for l in layers:
+            got = model.get_preactivations(inputs[l], l)
+            assert bool(((got.cpu().double() - want[l]).abs() <= tol[l]).all()), l
+
+    check(1)
+    for l in range(3):
+        model.encoder_module.encoders[l].weight.data[:, 7 + l].add_(1.5)
+    check(1)
+    check(1, 0)
+    pre, _ = model._encode_all_layers({1: inputs[1], 2: inputs[2]})
+    want, tol = _with_values(model, x)
+    for l in (1, 2):
+        assert bool(((pre[l].cpu().double() - want[l]).abs() <= tol[l]).all())
+    model.encoder_module.encoders[2].weight.data.neg_()
+    check(0, 1, 2)
+
+
 def test_training_of_a_quantised_model_is_refused(dev):
     model, inputs, x = _model(dev, T=40)
     targets = {l: v.clone() for l, v in inputs.items()}
