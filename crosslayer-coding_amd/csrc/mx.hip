@@ -607,8 +607,10 @@ __global__ __launch_bounds__(256, 2) void k_mx_project_few(FewArgs a, const OutT
 // 600 us, without loads 531, without stores 472, without both 406 (of which the products alone would be 281 at the 6.6 PFLOP/s that
 // the power limit leaves them on random operands).  On 16 x 8192 x 2048 x 16384: 2160 - 2230 us (4000 TFLOP/s); 4 products of
 // 8192^3: 960 us (4580).  Beside the stores it is bound by the LDS: per 128 of K its wavefronts read 96 KB from it and 32 KB are put
-// in, 1024 of its cycles at 128 bytes each, as many as the products themselves take at their full rate.  What did not help: groups
-// of 4, 16 or 32 feature tiles in the order of the tiles (3 - 5 us slower).
+// in, 1024 of its cycles at 128 bytes each, as many as the products themselves take at their full rate; and by the power limit: of
+// operands that are all zeros the first takes 496 us, the second 1818, and 4 products of 8192 x 4096 x 8192 428 us instead of 546.
+// What did not help: groups of 4, 16 or 32 feature tiles in the order of the tiles (3 - 5 us slower); wavefronts' priorities
+// (nothing); four wavefronts of 128 x 128 with the accumulators in the AGPRs (642 -> 701 us; nobody fills the waits).
 constexpr int TW = 8;                         // wavefronts
 constexpr int TROW = 128;                     // bytes of codes per row and stage
 // Of a buffer store, taken where the rows of the result begin with a cache line (LINES): its parts are whole lines, and past the caches
