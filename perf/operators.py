@@ -276,23 +276,18 @@ def work(case):
 _GRID4 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
-def _two_to(e):
-    """2^e in float64 from its bits, exact on every device (a library's power need not be)."""
-    return ((e.to(torch.int64) + 1023) << 52).view(torch.float64)
-
-
 def _values64(x, fmt):
     """What the codes of x stand for: the format's definition, value by value, in float64."""
     d = x.shape[-1]
     v = torch.nn.functional.pad(x.double(), (0, -d % BLOCK)).unflatten(-1, (-1, BLOCK))
     top = torch.frexp(v.abs().amax(-1, keepdim=True))[1] - 1                # floor(log2(largest)); 0 of a block of zeros
-    scale = _two_to((top - EMAX[fmt]).clamp(min=-127))
+    scale = torch.pow(2.0, (top - EMAX[fmt]).clamp(min=-127).double())
     v = v / scale
     m, sign = v.abs(), torch.sign(v)
     if fmt == "mxint8":
         q = torch.clamp(torch.round(m * 64), max=127) / 64
     elif fmt == "mxfp8":
-        quantum = _two_to((torch.frexp(m)[1] - 1).clamp(min=-6) - 3)
+        quantum = torch.pow(2.0, ((torch.frexp(m)[1] - 1).clamp(min=-6) - 3).double())
         q = torch.clamp(torch.round(m / quantum) * quantum, max=448.0)
     else:
         grid = torch.tensor(_GRID4, dtype=torch.float64, device=x.device)
@@ -308,11 +303,11 @@ def _stored64(codes, scales, fmt, d):
         q = torch.where(c >= 128, c - 256, c).double() / 64
     elif fmt == "mxfp8":
         e, m = (c >> 3) & 15, (c & 7).double()
-        q = torch.where(e == 0, m * 2.0 ** -9, (8 + m) * _two_to(e - 10)) * torch.where(c >= 128, -1.0, 1.0)
+        q = torch.where(e == 0, m * 2.0 ** -9, (8 + m) * torch.pow(2.0, (e - 10).double())) * torch.where(c >= 128, -1.0, 1.0)
     else:
         c = torch.stack((c % 16, c // 16), dim=-1).flatten(-2)
         q = torch.tensor(_GRID4 + tuple(-v for v in _GRID4), dtype=torch.float64, device=c.device)[c]
-    return (q.unflatten(-1, (-1, BLOCK)) * _two_to(scales.to(torch.int64) - 127).unsqueeze(-1)).flatten(-2)[..., :d]
+    return (q.unflatten(-1, (-1, BLOCK)) * torch.pow(2.0, scales.double() - 127).unsqueeze(-1)).flatten(-2)[..., :d]
 
 
 def exact(case, seed):
