@@ -38,10 +38,12 @@ class Encoder(nn.Module):
             ColumnParallelLinear(d, F, bias=True, process_group=process_group, device=device, dtype=dtype,
                                  weight_storage=self._w_slab[l], bias_storage=self._b_slab[l])
             for l in range(L))
-        # 4-bit copy of the weights (`quantise`), the parameters it was made from, and the fingerprints of their data
+        # 4-bit copy of the weights (`quantise`), the parameters it was made from, the fingerprints of their data, and whether
+        # these have been taken since the copy was made
         self._mx: Optional[mx.MXTensor] = None
         self._mx_keys: Optional[Tuple] = None
         self._mx_state: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+        self._mx_fresh = False
         self._mx_fmt: Optional[str] = None
         self.watch_parameter_data = True
 
@@ -95,7 +97,7 @@ class Encoder(nn.Module):
 
     def dequantise(self) -> None:
         """Project from the parameters again; the copy is given back."""
-        self._mx_fmt, self._mx, self._mx_keys, self._mx_state = None, None, None, None
+        self._mx_fmt, self._mx, self._mx_keys, self._mx_state, self._mx_fresh = None, None, None, None, False
 
     def quantised_weights(self) -> mx.MXTensor:
         """The copy, true to the parameters: made anew where a parameter's storage or version counter changed, and by the
@@ -117,11 +119,15 @@ class Encoder(nn.Module):
                 self._mx = mx.quantise(w.detach(), self._mx_fmt, out=out)
             # a capture only records: its replays quantise, and the next eager call does so again
             self._mx_keys = None if capturing else keys
-            self._mx_state = None
-        if self.watch_parameter_data and not (capturing and self._mx_state is None):
-            if self._mx_state is None:
+            self._mx_fresh = False
+        if self.watch_parameter_data and not (capturing and not self._mx_fresh):
+            # captured forwards have the fingerprints' addresses: they are written anew where they are, and live as long as the copy
+            if self._mx_state is None or self._mx_state[0].device != w.device:
                 self._mx_state = (torch.zeros(16 * L, dtype=torch.int64, device=w.device), torch.zeros(L, dtype=torch.int32, device=w.device))
+                self._mx_fresh = False
+            if not self._mx_fresh:
                 mx.refresh(w.detach(), self._mx, *self._mx_state, store_only=True)
+                self._mx_fresh = True
             else:
                 mx.refresh(w.detach(), self._mx, *self._mx_state, first=first, n=n)
         return self._mx if n is None else self._mx.narrow(first, n)

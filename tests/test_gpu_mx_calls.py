@@ -1,0 +1,79 @@
+"""Microscaled formats on the device: calls that earlier tests leave out.
+
+The forward of a quantised model between writes of every kind and replays, and the projection's paths that only large batches, rows
+already in codes or very wide rows take.  Bounds as in the tests of the operators: a sum of K exact products in float32 is within
+K 2^-23 of the sum of the magnitudes, the bias adds one addition, the type half a step."""
+import pytest
+import torch
+
+import crosslayer_coding_amd as cca
+from crosslayer_coding_amd import synth
+from oracle import mx_oracle as orc
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+# ---- a model whose encoder is quantised ----------------------------------------------------------------------------
+
+def _model(dev, T=40, dtype="bfloat16", fn="batchtopk", d=256, F=1024, L=3):
+    model, inputs, x = synth.build_model(synth.Workload("mx", 9, L, d, F, T, dtype, fn, 16, "per_layer", "none"), dev)
+    return model, inputs, x
+
+
+def _true(model, inputs, x):
+    """The pre-activations are those of the weights as they are now."""
+    w = torch.stack([e.weight.detach() for e in model.encoder_module.encoders]).cpu()
+    b = torch.stack([e.bias_param.detach() for e in model.encoder_module.encoders]).cpu().double().unsqueeze(1)
+    xq, wq = orc.round_trip(x.cpu(), "mxfp4"), orc.round_trip(w, "mxfp4")
+    want = xq @ wq.transpose(1, 2) + b
+    tol = (xq.abs() @ wq.abs().transpose(1, 2) + b.abs()) * (w.shape[-1] + 1) * 2.0 ** -23 + want.abs() * torch.finfo(model.dtype).eps / 2 * 1.01 + 1e-30
+    pre, _ = model._encode_all_layers(inputs)
+    for l in inputs:
+        assert bool(((pre[l].cpu().double() - want[l]).abs() <= tol[l]).all()), l
+
+
+def _capture(model, inputs):
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            model(inputs)
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = model(inputs)
+    return g, out
+
+
+@pytest.mark.parametrize("how", ["mul_", "load_state_dict"])
+def test_a_captured_forward_lives_through_writes_that_the_host_sees(dev, how):
+    """Capture, write, an eager forward on another stream, other tensors in the memory that is free now, replay."""
+    model, inputs, x = _model(dev)
+    model.quantise_encoder()
+    with torch.no_grad():
+        g, out = _capture(model, inputs)
+        at = [t.data_ptr() for t in model.encoder_module._mx_state]
+        for trial in range(3):
+            if how == "mul_":
+                model.encoder_module.encoders[trial].weight.mul_(-1.5)
+            else:
+                model.load_state_dict({k: v * 0.75 for k, v in model.state_dict().items()})
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                model(inputs)
+                others = [torch.full((n,), 7, dtype=torch.int32, device=dev) for n in (3, 48, 96, 128) for _ in range(8)]
+            torch.cuda.current_stream().wait_stream(s)
+            others += [torch.full((n,), 7, dtype=torch.int32, device=dev) for n in (3, 48, 96, 128) for _ in range(8)]
+            assert at == [t.data_ptr() for t in model.encoder_module._mx_state]
+            if trial == 2:
+                model.encoder_module.encoders[0].weight.data.neg_()         # seen by the replay alone
+            g.replay()
+            torch.cuda.synchronize()
+            got = {l: v.clone() for l, v in out.items()}
+            assert all(bool((t == 7).all()) for t in others)
+            want = model(inputs)
+            assert all(torch.equal(got[l], want[l]) for l in got), trial
+            _true(model, inputs, x)

@@ -1,0 +1,129 @@
+"""The 4-bit copy of a quantised encoder's weights: when it is made, looked at and kept, on the host.
+
+The device is played by lists of launches.  An eager launch runs at once; one under a capture is put down with what a graph
+would have of it - addresses, which keep nothing alive - and runs when it is replayed."""
+import weakref
+
+import numpy as np
+import pytest
+import torch
+
+import crosslayer_coding_amd as cca
+from crosslayer_coding_amd import encoder as encoder_module
+from oracle import mx_oracle as orc
+
+L, D, F = 3, 64, 40
+
+
+class Device:
+    def __init__(self):
+        self.recording = None
+        self.quantised = 0
+
+    def launch(self, run, *memory):
+        """``run(*memory)``; memory: tensors that the launch has the addresses of."""
+        if self.recording is None:
+            run(*memory)
+            return
+        refs = [weakref.ref(t) for t in memory]
+
+        def replay():
+            held = [r() for r in refs]
+            assert all(t is not None for t in held), "a captured launch goes to memory that was given back"
+            run(*held)
+
+        self.recording.append(replay)
+
+    def capture(self, call):
+        self.recording, graph = [], None
+        call()
+        graph, self.recording = self.recording, None
+        return graph
+
+    # ---- mx.quantise and mx.refresh, from the oracle; every element counts in these fingerprints
+    def quantise(self, x, fmt, out=None):
+        if out is None:
+            pitch, blocks = cca.mx.row_layout(x.shape[-1], fmt)
+            out = cca.MXTensor(torch.zeros(*x.shape[:-1], pitch, dtype=torch.uint8), torch.zeros(*x.shape[:-1], blocks, dtype=torch.uint8), fmt, x.shape[-1])
+
+        def run(codes, scales):
+            self.quantised += 1
+            c, s = orc.quantise(x, fmt)
+            codes.copy_(c), scales.copy_(s)
+
+        self.launch(run, out.codes, out.scales)
+        return out
+
+    def refresh(self, x, out, state, changed, store_only=False, first=0, n=None):
+        def run(codes, scales, state, changed):
+            for l in range(first, L if n is None else first + n):
+                line = state[16 * l:16 * l + 3]
+                assert int(line[0]) == 0 and int(line[1]) == 0, "sum and arrivals begin at zero"
+                now = int(np.frombuffer(x[l].contiguous().numpy().tobytes(), dtype=np.uint32).astype(np.int64).cumsum().sum() % (2 ** 62))
+                changed[l] = int(not store_only and int(line[2]) != now)
+                line[2] = now
+                if changed[l]:
+                    c, s = orc.quantise(x[l], "mxfp4")
+                    codes[l].copy_(c), scales[l].copy_(s)
+
+        self.launch(run, out.codes, out.scales, state, changed)
+
+
+@pytest.fixture
+def device(monkeypatch):
+    d = Device()
+    monkeypatch.setattr(encoder_module.mx, "quantise", d.quantise)
+    monkeypatch.setattr(encoder_module.mx, "refresh", d.refresh)
+    monkeypatch.setattr(encoder_module.nat, "require_device", lambda t, what: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: d.recording is not None)
+    return d
+
+
+@pytest.fixture
+def enc(device):
+    cfg = cca.CLTConfig(num_features=F, num_layers=L, d_model=D, batchtopk_k=4, clt_dtype="float32")
+    e = encoder_module.Encoder(cfg, None, torch.device("cpu"), torch.float32)
+    g = torch.Generator().manual_seed(3)
+    with torch.no_grad():
+        for lin in e.encoders:
+            lin.weight.copy_(torch.randn(F, D, generator=g))
+    e.quantise()
+    return e
+
+
+def _true(enc, layers=range(L)):
+    q = enc._mx
+    for l in layers:
+        codes, scales = orc.quantise(enc.encoders[l].weight.detach(), "mxfp4")
+        assert torch.equal(q.codes[l], codes) and torch.equal(q.scales[l], scales), l
+
+
+def _write(enc, l, how):
+    w = enc.encoders[l].weight
+    with torch.no_grad():
+        if how == "mul_":
+            w.mul_(-1.5)
+        elif how == "load_state_dict":
+            enc.load_state_dict({k: v * 0.5 for k, v in enc.state_dict().items()})
+        else:
+            w.data.mul_(2.0)
+
+
+@pytest.mark.parametrize("how", ["mul_", "load_state_dict"])
+@pytest.mark.parametrize("between", ["eager", "capture"])
+def test_fingerprints_outlive_the_writes_that_a_captured_forward_lives_through(device, enc, how, between):
+    enc.quantised_weights()
+    graph = device.capture(enc.quantised_weights)
+    for trial in range(2):
+        _write(enc, 1, how)
+        if between == "eager":
+            enc.quantised_weights()
+        else:
+            device.capture(enc.quantised_weights)
+            enc.quantised_weights()
+        _write(enc, 2, "data")
+        for launch in graph:
+            launch()
+        _true(enc)
+        enc.quantised_weights()
+        _true(enc)
