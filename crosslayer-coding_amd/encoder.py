@@ -118,18 +118,16 @@ class Encoder(nn.Module):
             with torch.no_grad():
                 self._mx = mx.quantise(w.detach(), self._mx_fmt, out=out)
             # a capture only records: its replays quantise, and the next eager call does so again
-            self._mx_keys = None if capturing else keys
-            self._mx_fresh = False
-        if self.watch_parameter_data and not (capturing and not self._mx_fresh):
-            # captured forwards have the fingerprints' addresses: they are written anew where they are, and live as long as the copy
-            if self._mx_state is None or self._mx_state[0].device != w.device:
-                self._mx_state = (torch.zeros(16 * L, dtype=torch.int64, device=w.device), torch.zeros(L, dtype=torch.int32, device=w.device))
-                self._mx_fresh = False
-            if not self._mx_fresh:
+            self._mx_keys, self._mx_fresh = None if capturing else keys, False
+            if not capturing:
+                # Fingerprints are taken of nothing but the weights that the codes were made of in this call, watched or not.  Captured
+                # forwards have their addresses: they are written anew where they are, and live as long as the copy.
+                if self._mx_state is None or self._mx_state[0].device != w.device:
+                    self._mx_state = (torch.zeros(16 * L, dtype=torch.int64, device=w.device), torch.zeros(L, dtype=torch.int32, device=w.device))
                 mx.refresh(w.detach(), self._mx, *self._mx_state, store_only=True)
                 self._mx_fresh = True
-            else:
-                mx.refresh(w.detach(), self._mx, *self._mx_state, first=first, n=n)
+        elif self.watch_parameter_data and self._mx_fresh:
+            mx.refresh(w.detach(), self._mx, *self._mx_state, first=first, n=n)
         return self._mx if n is None else self._mx.narrow(first, n)
 
     def project(self, layers: List[int], x: torch.Tensor, w: torch.Tensor, b: torch.Tensor, out: Optional[torch.Tensor] = None,

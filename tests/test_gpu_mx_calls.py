@@ -77,3 +77,18 @@ def test_a_captured_forward_lives_through_writes_that_the_host_sees(dev, how):
             want = model(inputs)
             assert all(torch.equal(got[l], want[l]) for l in got), trial
             _true(model, inputs, x)
+
+
+def test_a_write_while_nobody_watched_is_seen_when_somebody_does_again(dev):
+    model, inputs, x = _model(dev)
+    enc = model.encoder_module
+    with torch.no_grad():
+        enc.watch_parameter_data = False
+        model.quantise_encoder()
+        enc.encoders[1].weight.mul_(-1.5)
+        _true(model, inputs, x)
+        for lin in enc.encoders:
+            lin.weight.data.mul_(0.5)
+        enc.watch_parameter_data = True
+        model.get_preactivations(inputs[2], 2)
+        _true(model, inputs, x)

@@ -127,3 +127,33 @@ def test_fingerprints_outlive_the_writes_that_a_captured_forward_lives_through(d
         _true(enc)
         enc.quantised_weights()
         _true(enc)
+
+
+@pytest.mark.parametrize("layers", ["all", "one"])
+def test_a_write_while_nobody_watched_is_seen_when_somebody_does_again(device, enc, layers):
+    enc.watch_parameter_data = False
+    _write(enc, 1, "mul_")
+    enc.quantised_weights()                             # made without a look at the data
+    _true(enc)
+    for l in range(L):
+        _write(enc, l, "data")
+    enc.quantised_weights()
+    enc.watch_parameter_data = True
+    if layers == "one":
+        enc._quantised_slab(2, 1)
+        _true(enc, [2])
+    enc.quantised_weights()
+    _true(enc)
+
+
+def test_watching_from_the_first_copy_on_is_not_needed(device, enc):
+    enc.dequantise()
+    enc.watch_parameter_data = False
+    enc.quantise()
+    _write(enc, 0, "data")
+    enc.watch_parameter_data = True
+    enc.quantised_weights()
+    _true(enc)
+    before = device.quantised
+    enc.quantised_weights()
+    assert device.quantised == before
