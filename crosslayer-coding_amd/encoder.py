@@ -39,11 +39,11 @@ class Encoder(nn.Module):
                                  weight_storage=self._w_slab[l], bias_storage=self._b_slab[l])
             for l in range(L))
         # 4-bit copy of the weights (`quantise`), the parameters it was made from, the fingerprints of their data, and whether
-        # these have been taken since the copy was made
+        # these began as zeros (not yet where a capture made them)
         self._mx: Optional[mx.MXTensor] = None
         self._mx_keys: Optional[Tuple] = None
         self._mx_state: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
-        self._mx_fresh = False
+        self._mx_clear = False
         self._mx_fmt: Optional[str] = None
         self.watch_parameter_data = True
 
@@ -97,7 +97,7 @@ class Encoder(nn.Module):
 
     def dequantise(self) -> None:
         """Project from the parameters again; the copy is given back."""
-        self._mx_fmt, self._mx, self._mx_keys, self._mx_state, self._mx_fresh = None, None, None, None, False
+        self._mx_fmt, self._mx, self._mx_keys, self._mx_state, self._mx_clear = None, None, None, None, False
 
     def quantised_weights(self) -> mx.MXTensor:
         """The copy, true to the parameters: made anew where a parameter's storage or version counter changed, and by the
@@ -117,16 +117,19 @@ class Encoder(nn.Module):
             out = self._mx if self._mx is not None and self._mx.device == w.device and self._mx.shape == w.shape else None
             with torch.no_grad():
                 self._mx = mx.quantise(w.detach(), self._mx_fmt, out=out)
+            # Fingerprints are taken of nothing but the weights that the codes were made of in this call or replay, watched or not.
+            # Captured forwards have their addresses: they are written anew where they are, and live as long as the copy.
+            if self._mx_state is None or self._mx_state[0].device != w.device:
+                self._mx_state = (torch.zeros(16 * L, dtype=torch.int64, device=w.device), torch.zeros(L, dtype=torch.int32, device=w.device))
+                self._mx_clear = not capturing
+            elif not self._mx_clear:                        # no replay need have filled them with zeros
+                for t in self._mx_state:
+                    t.zero_()
+                self._mx_clear = not capturing
+            mx.refresh(w.detach(), self._mx, *self._mx_state, store_only=True)
             # a capture only records: its replays quantise, and the next eager call does so again
-            self._mx_keys, self._mx_fresh = None if capturing else keys, False
-            if not capturing:
-                # Fingerprints are taken of nothing but the weights that the codes were made of in this call, watched or not.  Captured
-                # forwards have their addresses: they are written anew where they are, and live as long as the copy.
-                if self._mx_state is None or self._mx_state[0].device != w.device:
-                    self._mx_state = (torch.zeros(16 * L, dtype=torch.int64, device=w.device), torch.zeros(L, dtype=torch.int32, device=w.device))
-                mx.refresh(w.detach(), self._mx, *self._mx_state, store_only=True)
-                self._mx_fresh = True
-        elif self.watch_parameter_data and self._mx_fresh:
+            self._mx_keys = None if capturing else keys
+        elif self.watch_parameter_data:
             mx.refresh(w.detach(), self._mx, *self._mx_state, first=first, n=n)
         return self._mx if n is None else self._mx.narrow(first, n)
 

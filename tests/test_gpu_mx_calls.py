@@ -92,3 +92,59 @@ def test_a_write_while_nobody_watched_is_seen_when_somebody_does_again(dev):
         enc.watch_parameter_data = True
         model.get_preactivations(inputs[2], 2)
         _true(model, inputs, x)
+
+
+def test_a_replay_that_makes_the_copy_takes_its_fingerprints_too(dev):
+    """Weights put in for one replay and taken out again, past the version counters; the graph was captured right after a write."""
+    model, inputs, x = _model(dev)
+    model.quantise_encoder()
+    weight = model.encoder_module.encoders[1].weight
+    with torch.no_grad():
+        model(inputs)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            model(inputs)
+        torch.cuda.current_stream().wait_stream(s)
+        weight.mul_(-0.5)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = model(inputs)
+        for trial in range(3):
+            want = {l: v.clone() for l, v in model(inputs).items()}
+            kept = weight.detach().clone()
+            weight.data.mul_(0.3)
+            g.replay()
+            torch.cuda.synchronize()
+            got = {l: v.clone() for l, v in out.items()}
+            other = model(inputs)
+            assert all(torch.equal(got[l], other[l]) for l in got)
+            g.replay()
+            weight.data.copy_(kept)
+            again = model(inputs)
+            assert all(torch.equal(again[l], want[l]) for l in want), trial
+            _true(model, inputs, x)
+
+
+def test_a_copy_that_is_first_made_under_a_capture(dev):
+    model, inputs, x = _model(dev)
+    with torch.no_grad():
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            model(inputs)
+        torch.cuda.current_stream().wait_stream(s)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            model.quantise_encoder()
+            out = model(inputs)
+        want = {l: v.clone() for l, v in model(inputs).items()}
+        _true(model, inputs, x)
+        for trial in range(3):
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(out[l], want[l]) for l in want), trial
+            again = model(inputs)
+            assert all(torch.equal(again[l], want[l]) for l in want), trial
+        model.encoder_module.encoders[0].weight.data.neg_()
+        _true(model, inputs, x)

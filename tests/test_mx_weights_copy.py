@@ -157,3 +157,35 @@ def test_watching_from_the_first_copy_on_is_not_needed(device, enc):
     before = device.quantised
     enc.quantised_weights()
     assert device.quantised == before
+
+
+def test_a_replay_that_makes_the_copy_takes_its_fingerprints_too(device, enc):
+    """Weights put in for one replay and taken out again, all past the version counters."""
+    _write(enc, 1, "mul_")
+    graph = device.capture(enc.quantised_weights)       # right after a write: the graph quantises
+    enc.quantised_weights()
+    kept = enc.encoders[1].weight.detach().clone()
+    enc.encoders[1].weight.data.mul_(0.3)
+    for launch in graph:
+        launch()
+    _true(enc)
+    enc.encoders[1].weight.data.copy_(kept)
+    enc.quantised_weights()
+    _true(enc)
+
+
+def test_a_copy_that_is_first_made_under_a_capture(device, enc):
+    enc.dequantise()
+    enc._mx_fmt = "mxfp4"                               # as after a move to another device: there is no copy there yet
+    graphs = [device.capture(enc.quantised_weights) for _ in range(2)]
+    for trial in range(2):
+        _write(enc, 1, "data")
+        for launch in graphs[trial]:
+            launch()
+        _true(enc)
+    _write(enc, 2, "data")
+    enc.quantised_weights()
+    _true(enc)
+    _write(enc, 0, "data")
+    enc.quantised_weights()
+    _true(enc)
