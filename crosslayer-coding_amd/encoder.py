@@ -92,8 +92,14 @@ class Encoder(nn.Module):
             raise ValueError(f"the projection takes mxfp4 weights, asked for {fmt!r}")
         nat.require_device(self.first_weight(), "quantise")
         mx.row_layout(self.config.d_model, fmt)
+        was = self._mx_fmt
         self._mx_fmt = fmt
-        self.quantised_weights()
+        try:
+            self.quantised_weights()
+        except Exception:
+            if was is None:                                 # the projection stays with the parameters
+                self.dequantise()
+            raise
 
     def dequantise(self) -> None:
         """Project from the parameters again; the copy is given back."""

@@ -189,3 +189,27 @@ def test_a_copy_that_is_first_made_under_a_capture(device, enc):
     _write(enc, 0, "data")
     enc.quantised_weights()
     _true(enc)
+
+
+def test_a_copy_that_cannot_be_made_leaves_the_encoder_as_it_was(device, enc, monkeypatch):
+    def no_memory(*args, **kw):
+        raise torch.cuda.OutOfMemoryError("no memory for the copy")
+
+    enc.dequantise()
+    with monkeypatch.context() as m:
+        m.setattr(encoder_module.mx, "quantise", no_memory)
+        with pytest.raises(torch.cuda.OutOfMemoryError):
+            enc.quantise()
+        assert enc.quantised is None and enc._mx is None
+    enc.quantise()
+    _true(enc)
+    with pytest.raises(ValueError):
+        enc.quantise("mxfp8")
+    _write(enc, 0, "mul_")
+    with monkeypatch.context() as m:                    # a copy that is there stays in use, and is made anew when it can be
+        m.setattr(encoder_module.mx, "quantise", no_memory)
+        with pytest.raises(torch.cuda.OutOfMemoryError):
+            enc.quantise()
+    assert enc.quantised == "mxfp4"
+    enc.quantised_weights()
+    _true(enc)
