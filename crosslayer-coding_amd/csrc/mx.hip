@@ -15,6 +15,7 @@
 namespace {
 
 constexpr int MX_THREADS = 256;
+constexpr int64_t MX_MAX_ROWS = 1LL << 40;  // of a store or an output, per layer: far more than memory holds, and their bytes are counted with 64 bits
 constexpr int64_t MX_MAX_WIDTH = 262144;    // elements of a row: the pieces of a workgroup's rows are told apart with 32 bits
 
 // The tiles of the projection: MX_BM tokens (four wavefronts of MX_MG groups of 16) x TN features, K in stages of TBLOCKS blocks.
@@ -1201,7 +1202,7 @@ int launch_mx_project(const MxPlan &p, const void *x, const void *xc, int64_t x_
 // sizes that every entry point asks for
 int mx_sizes(int64_t L, int64_t n, int64_t d, int64_t rows) {
   if (L <= 0 || n < 0 || d <= 0 || rows < 0) return CLT_ERR_ARG;
-  if (L > 32767 || d > MX_MAX_WIDTH || n > 2147483647LL || rows > (1LL << 40)) return CLT_ERR_RANGE;
+  if (L > 32767 || d > MX_MAX_WIDTH || n > 2147483647LL || rows > MX_MAX_ROWS) return CLT_ERR_RANGE;
   return CLT_OK;
 }
 
@@ -1258,7 +1259,7 @@ extern "C" int clt_mx_cache_write(const void *x, const void *tgt, int64_t layer_
   if (const int rc = mx_sizes(L, n, d, rows)) return rc;
   if (n == 0) return CLT_OK;
   if (!x || !tgt || !codes || !scales || row_stride < d || layer_stride < 0) return CLT_ERR_ARG;
-  if (row_index ? !owner : (first < 0 || first + n > rows)) return CLT_ERR_ARG;
+  if (row_index ? !owner : (first < 0 || n > rows || first > rows - n)) return CLT_ERR_ARG;
   if (!clt_aligned16(codes)) return CLT_ERR_ALIGN;
   const MxRows r{row_index, index_bits == 64, first, rows, row_index ? owner : nullptr};
   hipStream_t s = (hipStream_t)stream;
@@ -1278,10 +1279,11 @@ extern "C" int clt_mx_cache_read(const void *codes, const uint8_t *scales, int64
   if (!mx_format(fmt) || (row_index && index_bits != 32 && index_bits != 64)) return CLT_ERR_ARG;
   if (norm_mode < CLT_DENORM_NONE || norm_mode > CLT_DENORM_SCALE) return CLT_ERR_ARG;
   if (const int rc = mx_sizes(L, n, d, rows)) return rc;
-  if (T < 0 || out_row0 < 0 || out_row0 + n > T) return CLT_ERR_ARG;
+  if (T < 0 || out_row0 < 0 || n > T || out_row0 > T - n) return CLT_ERR_ARG;
+  if (T > MX_MAX_ROWS) return CLT_ERR_RANGE;
   if (n == 0) return CLT_OK;
   if (!codes || !scales || !x_out || !tgt_out || rows == 0) return CLT_ERR_ARG;
-  if (!row_index && (first < 0 || first + n > rows)) return CLT_ERR_ARG;
+  if (!row_index && (first < 0 || n > rows || first > rows - n)) return CLT_ERR_ARG;
   if (!clt_aligned16(codes)) return CLT_ERR_ALIGN;
   const MxRows r{row_index, index_bits == 64, first, rows, nullptr};
   const MxNorm nm{norm_mode, mean_in, std_in, mean_tg, std_tg, (float)scale};

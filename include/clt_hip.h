@@ -889,7 +889,7 @@ int clt_feed_gather(const void *src, int src_dtype, int64_t src_rows, int64_t sr
  *   CLT_MXINT8   32 bytes per block   two's complement in 64ths, -127/64 .. 127/64
  * A row of d elements has ceil(d / 32) blocks (the last one filled up with zeros): clt_mx_row_bytes(d, fmt) bytes of codes
  * (0: not a format) and ceil(d / 32) bytes of scales; rows follow one another without gaps, codes begin 16-byte aligned
- * (else CLT_ERR_ALIGN).  d up to 262144, at most 2^31 - 1 rows a call.
+ * (else CLT_ERR_ALIGN).  d up to 262144, at most 2^31 - 1 rows a call, stores and outputs (rows, T) of up to 2^40 rows (CLT_ERR_RANGE).
  *
  * clt_mx_quantise / clt_mx_dequantise: n rows of d elements (dtype CLT_F32 / CLT_BF16 / CLT_F16), row_stride elements
  *   apart, to codes and scales and back (fp32, one rounding to dtype).
