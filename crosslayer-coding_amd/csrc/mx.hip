@@ -15,6 +15,7 @@
 namespace {
 
 constexpr int MX_THREADS = 256;
+constexpr int64_t MX_MAX_GROUPS = (1 << 24) - 1;   // workgroups of 256 threads along one axis: a launch takes fewer than 2^32 threads there
 constexpr int64_t MX_MAX_ROWS = 1LL << 40;  // of a store or an output, per layer: far more than memory holds, and their bytes are counted with 64 bits
 constexpr int64_t MX_MAX_WIDTH = 262144;    // elements of a row: the pieces of a workgroup's rows are told apart with 32 bits
 
@@ -1026,7 +1027,7 @@ template <typename T, int FMT>
 int launch_mx_write(const void *src0, const void *src1, int64_t layer_stride, int64_t row_stride, int64_t L, int kinds, int64_t n, int64_t d,
                     uint32_t blocks, const MxRows &rows, void *codes, uint8_t *scales, hipStream_t s) {
   const int64_t groups = clt_ceil_div(n * (int64_t)(blocks * 2), MX_THREADS);
-  if (groups > 2147483647LL) return CLT_ERR_RANGE;
+  if (groups > MX_MAX_GROUPS) return CLT_ERR_RANGE;
   const dim3 grid((unsigned)groups, (unsigned)(L * kinds));
   const MxWrite a{src0, src1, layer_stride, row_stride, n, d, kinds, blocks, mx_magic(blocks * 2), rows, (uint8_t *)codes, scales};
   if (mx_write_vec<T>(src0, src1, layer_stride, row_stride, d)) k_mx_write<T, FMT, true><<<grid, MX_THREADS, 0, s>>>(a);
@@ -1059,7 +1060,7 @@ int launch_mx_read(const void *codes, const uint8_t *scales, const MxRows &rows,
   const uint32_t blocks = (uint32_t)clt_ceil_div(d, 32), pieces = (uint32_t)(vec ? d / E : clt_ceil_div(d, 8));
   const bool many = vec && L * kinds * clt_ceil_div(n, MX_U) * pieces >= MX_MANY;
   const int64_t apart = many ? clt_ceil_div(n, MX_U) : n, groups = clt_ceil_div(apart * (int64_t)pieces, MX_THREADS);
-  if (groups > 2147483647LL) return CLT_ERR_RANGE;
+  if (groups > MX_MAX_GROUPS) return CLT_ERR_RANGE;
   const dim3 grid((unsigned)groups, (unsigned)(L * kinds));
 #define CLT_MXR(VEC, U, LINES)                                                                                                             \
   k_mx_read<OutT, FMT, VEC, U, LINES><<<grid, MX_THREADS, 0, s>>>((const uint8_t *)codes, scales, rows, n, apart, d, blocks, pieces,           \
@@ -1153,7 +1154,7 @@ int launch_mx_project(const MxPlan &p, const void *x, const void *xc, int64_t x_
                       uint8_t *ws, void *pre, int64_t T, int64_t d, int64_t F, int64_t L, int64_t bs, int64_t ps, int64_t pre_row, hipStream_t s) {
   if (p.tiles) {
     const int64_t total = p.tm * p.tn * L;
-    if (total > 1073741824LL || p.tn * p.stages > 1073741824LL || p.tm * p.stages > 1073741824LL) return CLT_ERR_RANGE;
+    if (total > 1073741824LL || p.tn * p.stages + (x ? clt_ceil_div(T * p.padded * 2, MX_THREADS) : 0) > MX_MAX_GROUPS) return CLT_ERR_RANGE;
     const int grid = mx_grid(total);
     if (grid <= 0) return CLT_ERR_LAUNCH;
     const MxSide side{wsc, ws + p.ws, bias, (float *)(ws + p.bias), (int)F, (int)p.blocks, (int)p.stages, bs};

@@ -889,7 +889,8 @@ int clt_feed_gather(const void *src, int src_dtype, int64_t src_rows, int64_t sr
  *   CLT_MXINT8   32 bytes per block   two's complement in 64ths, -127/64 .. 127/64
  * A row of d elements has ceil(d / 32) blocks (the last one filled up with zeros): clt_mx_row_bytes(d, fmt) bytes of codes
  * (0: not a format) and ceil(d / 32) bytes of scales; rows follow one another without gaps, codes begin 16-byte aligned
- * (else CLT_ERR_ALIGN).  d up to 262144, at most 2^31 - 1 rows a call, stores and outputs (rows, T) of up to 2^40 rows (CLT_ERR_RANGE).
+ * (else CLT_ERR_ALIGN).  d up to 262144, at most 2^31 - 1 rows a call, stores and outputs (rows, T) of up to 2^40 rows; a launch
+ * takes fewer than 2^32 threads, which n * ceil(d / 32) < 2^30 always fits (else CLT_ERR_RANGE).
  *
  * clt_mx_quantise / clt_mx_dequantise: n rows of d elements (dtype CLT_F32 / CLT_BF16 / CLT_F16), row_stride elements
  *   apart, to codes and scales and back (fp32, one rounding to dtype).
@@ -915,7 +916,8 @@ int clt_feed_gather(const void *src, int src_dtype, int64_t src_rows, int64_t sr
  *   [L][T][d] values of dtype, layers x_layer_stride apart, which the call quantises, when x_scales is NULL; else its
  *   codes and scales [L][T].  pre rows are pre_row_stride >= F elements apart, layers pre_layer_stride.
  *   What clt_encode computes from 16- or 32-bit operands (clt/models/parallel.py:286).  workspace: 16-byte aligned,
- *   clt_mx_encode_workspace_bytes (may be 0 when x comes quantised).  T up to 16 * 65535, F up to 2^30, L up to 32767.
+ *   clt_mx_encode_workspace_bytes (may be 0 when x comes quantised).  T up to 16 * 65535, F up to 2^30, L up to 32767,
+ *   (T + F / 4) * ceil(d / 32) below 2^30 (CLT_ERR_RANGE).
  */
 #define CLT_MXFP4 0
 #define CLT_MXFP8 1
