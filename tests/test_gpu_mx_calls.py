@@ -148,3 +148,71 @@ def test_a_copy_that_is_first_made_under_a_capture(dev):
             assert all(torch.equal(again[l], want[l]) for l in want), trial
         model.encoder_module.encoders[0].weight.data.neg_()
         _true(model, inputs, x)
+
+
+# ---- the projection's paths ----------------------------------------------------------------------------------------
+
+def _whole_numbers(shape, top, seed):
+    """Small whole numbers, one element of each block fixed so that every block's scale is 1, times a scale per block."""
+    g = torch.Generator().manual_seed(seed)
+    v = torch.randint(-3, 4, shape, generator=g).float()
+    v[..., top::32] = 4.0
+    blocks = torch.tensor([1.0, 2.0, 0.5, 8.0])[torch.randint(0, 4, (*shape[:-1], -(-shape[-1] // 32)), generator=g)]
+    return v * blocks.repeat_interleave(32, dim=-1)[..., :shape[-1]]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("F", [4096, 4100])
+@pytest.mark.parametrize("d", [512, 640, 768, 1024, 2048])
+def test_project_of_several_tiles_a_workgroup(dev, dtype, F, d):
+    """576 and 612 tiles of 2 to 8 stages: a workgroup takes a second and a third one, whose stages follow each other while the tile
+    before leaves.  Every partial sum is a multiple of 1/4 below 2^22, so sums are exact in any order and the results are theirs,
+    rounded once.  F = 4096: rows of whole cache lines."""
+    L, T = 4, 2100
+    w = cca.mx.quantise(_whole_numbers((L, F, d), 1, 1).to(dev))
+    b = (torch.arange(L * F).reshape(L, F) % 200 - 100).to(dtype).to(dev)
+    w64 = w.dequantise().double()
+    for trial in range(2):
+        x = _whole_numbers((L, T, d), 0, 2 + trial).to(dtype).to(dev)
+        out = torch.full((L, T, F), float("nan"), dtype=dtype, device=dev)
+        cca.mx.project(x, w, b, out=out)
+        for l in range(L):
+            want = torch.mm(x[l].double(), w64[l].t().contiguous()) + b[l].double()
+            assert torch.equal(out[l], want.to(dtype)), (trial, l)
+    for _ in range(3):
+        assert torch.equal(cca.mx.project(x, w, b), out)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("L,T,F,d", [(2, 300, 520, 640), (1, 512, 512, 512), (2, 256, 300, 768), (3, 70, 1000, 96), (1, 1000, 260, 2048), (4, 2100, 4096, 768)])
+def test_project_of_rows_in_codes_by_tiles(dev, dtype, L, T, F, d):
+    """Rows that come in codes, whole tiles of whole stages and others, give what the same rows quantised on the way in give."""
+    g = torch.Generator().manual_seed(T + d)
+    x = torch.randn(L, T, d, generator=g).to(dtype).to(dev)
+    w = cca.mx.quantise((torch.randn(L, F, d, generator=g) / d ** 0.5).to(dev))
+    b = torch.randn(L, F, generator=g).to(dtype).to(dev)
+    xq = cca.mx.quantise(x)
+    out = torch.full((L, T, F), float("nan"), dtype=dtype, device=dev)
+    cca.mx.project(xq, w, b, out=out)
+    assert torch.equal(out, cca.mx.project(x, w, b))
+    x64, w64 = xq.dequantise().double(), w.dequantise().double()
+    for l in range(L):
+        want = torch.mm(x64[l], w64[l].t().contiguous()) + b[l].double()
+        mag = torch.mm(x64[l].abs(), w64[l].abs().t().contiguous()) + b[l].double().abs()
+        tol = mag * (d + 1) * 2.0 ** -23 + want.abs() * torch.finfo(dtype).eps / 2 * 1.01 + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+        assert bool(((out[l].double() - want).abs() <= tol).all()), l
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("L,T,F,d", [
+    (1, 1, 100, 9700), (2, 20, 100, 10016), (1, 70, 37, 9700), (1, 5, 301, 12000),      # rows that LDS does not hold
+    (1, 40, 100, 2048), (2, 33, 1000, 2000), (1, 16, 130, 9000)])                       # and those that take more than 64 KB of it
+def test_project_of_few_tokens_and_wide_rows(dev, dtype, L, T, F, d):
+    x = _whole_numbers((L, T, d), 0, T).to(dtype)
+    w = _whole_numbers((L, F, d), 1, F)
+    b = (torch.arange(L * F).reshape(L, F) % 200 - 100).to(dtype)
+    want = (torch.bmm(x.double(), w.double().transpose(1, 2).contiguous()) + b.double().unsqueeze(1)).to(dtype)
+    wq = cca.mx.quantise(w.to(dev))
+    got = cca.mx.project(x.to(dev), wq, b.to(dev))
+    assert torch.equal(got.cpu(), want)
+    assert torch.equal(cca.mx.project(cca.mx.quantise(x.to(dev)), wq, b.to(dev)).cpu(), want)
