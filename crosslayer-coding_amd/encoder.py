@@ -225,7 +225,8 @@ class Encoder(nn.Module):
 
     def prepare_slab(self, inputs: Dict[int, torch.Tensor]):
         """(sorted layers, x [n, T, d], weights [n, F, d], biases [n, F]) of the given layers, or
-        None when some input needs the per-layer fallbacks."""
+        None when some input needs the per-layer fallbacks.  Quantised, the weights are those of all layers as they lie: `project`
+        multiplies the 4-bit ones and copies no others."""
         layers = sorted(inputs.keys())
         if not layers:
             return None
@@ -250,7 +251,7 @@ class Encoder(nn.Module):
             ws, bs = w, b
         else:
             idx = torch.tensor(layers, device=w.device)
-            ws, bs = w.index_select(0, idx), b.index_select(0, idx)
+            ws, bs = w if self._mx_fmt is not None else w.index_select(0, idx), b.index_select(0, idx)
         return layers, x_slab, ws, bs
 
 

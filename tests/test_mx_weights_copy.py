@@ -213,3 +213,21 @@ def test_a_copy_that_cannot_be_made_leaves_the_encoder_as_it_was(device, enc, mo
     assert enc.quantised == "mxfp4"
     enc.quantised_weights()
     _true(enc)
+
+
+@pytest.mark.parametrize("layers", [[1], [0, 1], [0, 2]])
+def test_some_layers_of_a_quantised_encoder_copy_no_weights_that_nobody_reads(device, enc, monkeypatch, layers):
+    inputs = {l: torch.randn(5, D) for l in layers}
+    slab = enc._w_slab.untyped_storage().data_ptr()
+    enc.dequantise()
+    assert enc.prepare_slab(inputs)[2].shape == (len(layers), F, D)
+    enc.quantise()
+    got, x, w, b = enc.prepare_slab(inputs)
+    assert got == layers and x.shape == (len(layers), 5, D)
+    assert w.untyped_storage().data_ptr() == slab
+    assert torch.equal(b, enc._b_slab[layers])
+    seen = []
+    monkeypatch.setattr(encoder_module.mx, "project", lambda x, q, b, out=None, ws=None: seen.append(q) or torch.zeros(*x.shape[:2], F))
+    _, pre = enc.encode_slab(inputs)
+    codes, scales = orc.quantise(enc._w_slab[layers].detach(), "mxfp4")
+    assert pre.shape == (len(layers), 5, F) and torch.equal(seen[0].codes, codes) and torch.equal(seen[0].scales, scales)
