@@ -225,10 +225,12 @@ class CrossLayerTranscoder(BaseTranscoder):
     # ---- 4-bit encoder -------------------------------------------------------------------------
     def quantise_encoder(self, fmt: str = "mxfp4") -> None:
         """Compute pre-activations from 4-bit weights and inputs from here on (inference: forward, activations, evaluation, theta
-        estimation).  The parameters and checkpoints stay as they are, and what is written to them shows in the next forward;
-        ``dequantise_encoder()`` goes back.  Selection and decode are the same; training entry points raise meanwhile.  Captured
-        forwards use the 4-bit copy and are replayed only while it is there; forwards on several streams at once need the caller's
-        ordering, since each looks whether the copy is up to date."""
+        estimation).  The parameters and checkpoints stay as they are; ``dequantise_encoder()`` goes back.  Selection and decode are
+        the same; training entry points raise meanwhile.  Writes to the weights show in the next forward: those that a version
+        counter or a storage pointer shows always, those through ``.data`` by samples of every row - a matrix, a whole row or
+        column always, a few scattered elements possibly not: call this again after such a write, it makes the copy anew.
+        Captured forwards use the 4-bit copy and are replayed only while it is there; forwards on several streams at once need the
+        caller's ordering, since each looks whether the copy is up to date."""
         self._sync_device()
         self.encoder_module.quantise(fmt)
 

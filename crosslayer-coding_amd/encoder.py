@@ -87,13 +87,14 @@ class Encoder(nn.Module):
         return self._mx_fmt
 
     def quantise(self, fmt: str = "mxfp4") -> None:
-        """Project from a 4-bit copy of the weights from here on (`mx.project`); the parameters stay as they are."""
+        """Project from a 4-bit copy of the weights from here on (`mx.project`); the parameters stay as they are.  Called again, it
+        makes the copy anew where it lies."""
         if fmt != "mxfp4":
             raise ValueError(f"the projection takes mxfp4 weights, asked for {fmt!r}")
         nat.require_device(self.first_weight(), "quantise")
         mx.row_layout(self.config.d_model, fmt)
         was = self._mx_fmt
-        self._mx_fmt = fmt
+        self._mx_fmt, self._mx_keys = fmt, None
         try:
             self.quantised_weights()
         except Exception:
@@ -107,8 +108,9 @@ class Encoder(nn.Module):
 
     def quantised_weights(self) -> mx.MXTensor:
         """The copy, true to the parameters: made anew where a parameter's storage or version counter changed, and by the
-        device itself for layers whose data alone did (``weight.data.fill_(...)``: every row and column of a weight is looked
-        at; ``watch_parameter_data`` = False leaves that out)."""
+        device itself for layers whose data alone did (``weight.data.fill_(...)``).  Of the data 64 bytes of every row are looked at, at
+        places that go round: a write past the version counter to a matrix, a whole row or (of d_model / 16 features or more) column shows, one to a few
+        scattered elements may not until `quantise` is called again.  ``watch_parameter_data`` = False leaves the look out."""
         self.stacked()
         return self._quantised_slab()
 

@@ -216,3 +216,16 @@ def test_project_of_few_tokens_and_wide_rows(dev, dtype, L, T, F, d):
     got = cca.mx.project(x.to(dev), wq, b.to(dev))
     assert torch.equal(got.cpu(), want)
     assert torch.equal(cca.mx.project(cca.mx.quantise(x.to(dev)), wq, b.to(dev)).cpu(), want)
+
+
+def test_quantise_again_shows_a_write_that_the_samples_miss(dev):
+    """Of a row 32 elements of 16 bits are looked at, of the first row the first ones."""
+    model, inputs, x = _model(dev)
+    model.quantise_encoder()
+    with torch.no_grad():
+        _true(model, inputs, x)
+        model.encoder_module.encoders[1].weight.data[0, 100] = 50.0
+        model.quantise_encoder()
+        _true(model, inputs, x)
+        model.encoder_module.encoders[2].weight[5, 77] = -50.0       # not past the version counter: shows by itself
+        _true(model, inputs, x)

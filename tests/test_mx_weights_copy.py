@@ -231,3 +231,15 @@ def test_some_layers_of_a_quantised_encoder_copy_no_weights_that_nobody_reads(de
     _, pre = enc.encode_slab(inputs)
     codes, scales = orc.quantise(enc._w_slab[layers].detach(), "mxfp4")
     assert pre.shape == (len(layers), 5, F) and torch.equal(seen[0].codes, codes) and torch.equal(seen[0].scales, scales)
+
+
+def test_quantise_again_makes_the_copy_anew_where_it_is(device, enc):
+    """For writes that a look at samples of the data may miss; captured forwards go on with the copy."""
+    graph = device.capture(enc.quantised_weights)
+    at, before = enc._mx.codes.data_ptr(), device.quantised
+    enc.quantise()
+    assert device.quantised == before + 1 and enc._mx.codes.data_ptr() == at
+    _write(enc, 0, "data")
+    for launch in graph:
+        launch()
+    _true(enc)
