@@ -208,8 +208,9 @@ template <typename T, int FMT, bool VEC> __global__ __launch_bounds__(MX_THREADS
 // workgroup compares and stores.
 // state: [L][16], a 128-byte line per layer: sum, workgroups that have arrived, fingerprint.
 //
-// 12 x 24576 rows of 768 bf16: 19 MB in 64-byte pieces, 21 us, of a layer's 64 workgroups with six loads in flight a lane; bound by
-// the latency of six rounds.  Eight workgroups a layer, one column a round: 196 us.
+// 12 x 24576 rows of 768 bf16: 19 MB in 64-byte pieces, 21 us (0.9 TB/s), of a layer's 64 workgroups; bound by the latency of six
+// rounds, since each load of a lane lies behind a branch and is waited for before the next.  Eight workgroups a layer, one column a
+// round: 196 us.
 constexpr int WATCH_BLOCKS = 64, WATCH_ROWS = WATCH_BLOCKS * 64;
 template <typename T>
 __global__ __launch_bounds__(256) void k_mx_watch(const T *__restrict__ src, int64_t layer_stride, int64_t n, int64_t d,
@@ -319,8 +320,9 @@ __device__ __forceinline__ float mx_quotient(float a, float s, float r) {
 
 // A thread gives out 16 bytes of U rows: E elements from one place on.  LINES: rows of the result are whole cache lines, so that
 // a wavefront's stores are too; they go past the caches, which would hold back the reads behind them.  12 x 24576 rows of 768 from
-// mxfp4 to bf16: 80 us, and 106 through the caches; 16 layers of 3001 x 2048 rows drawn from mxfp4 to float32, inputs and targets: 124
-// and 231 us.  Two rows a thread: four take 131 us on the second of these.
+// mxfp4 to bf16: 80 us where the codes are in the memory-side cache from the pass before and 105 where they come from memory, through the
+// caches 109 and 108; 16 layers of 3001 x 2048 rows drawn from mxfp4 to float32, inputs and targets: 121 us for rows that were just
+// read, 210 for others, through the caches 240 and 239.  Two rows a thread: four take 131 us on the second of these, on rows just read.
 template <typename OutT, int FMT, bool VEC, int U, bool LINES>
 __global__ __launch_bounds__(MX_THREADS) void k_mx_read(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, MxRows rows,
                                                         int64_t n, int64_t rows_apart, int64_t d, uint32_t blocks, uint32_t pieces,
@@ -444,6 +446,12 @@ __device__ __forceinline__ mx_f32x4_t mx_mma2(const mx_f32x4_t &c, const uint4 &
 // SRC says where x comes from: FEW_VALUES are quantised into LDS by every workgroup, FEW_CODES copied there; FEW_WIDE rows do not
 // fit and are read as they are used.  Rows past the end repeat the last one and store nothing, blocks past the end count as zeros.
 constexpr int FEW_VALUES = 0, FEW_CODES = 1, FEW_WIDE = 2;
+// K is filled up to whole runs of FEW_STEPS steps of 128, whose loads and products behind the end are in vain: with three nothing at
+// d = 768 and 1536, an eighth at 1024 and 2048, a fifth at 640, a half at 256 and 512.  Three were chosen at d = 768;
+// over other widths two are as fast or faster, but for d = 9473 .. 9600, whose rows then no longer fit into LDS (4 layers, F 4096,
+// one token, d 9536: 29 us with three, 64 with two).  One token of 12 layers with 120 MB of weights in all, us with three / two steps:
+// d 256 38 / 31, 512 38 / 29, 640 27 / 27, 768 26 / 24, 1024 42 / 38, 1536 32 / 31, 2048 54 / 48, 4096 36 / 35 (above 1024 x has a
+// launch of its own, MX_FEW_VALUES).
 constexpr int FEW_STEPS = 3, FEW_NF = 2, FEW_TN = 4 * 16 * FEW_NF;   // features of a workgroup
 constexpr int FEW_LDS = 80 * 1024;                                   // two workgroups per CU at least
 
@@ -606,11 +614,15 @@ __global__ __launch_bounds__(256, 2) void k_mx_project_few(FewArgs a, const OutT
 // so the waits for loads allow for the stores sent behind them.
 //
 // Measured on 12 x 4096 x 768 x 24576, bf16 out (2.42 GB: 405 - 450 us for a kernel that does nothing but store these tiles):
-// 600 us, without loads 531, without stores 472, without both 406 (of which the products alone would be 281 at the 6.6 PFLOP/s that
-// the power limit leaves them on random operands).  On 16 x 8192 x 2048 x 16384: 2160 - 2230 us (4000 TFLOP/s); 4 products of
-// 8192^3: 960 us (4580).  Beside the stores it is bound by the LDS: per 128 of K its wavefronts read 96 KB from it and 32 KB are put
-// in, 1024 of its cycles at 128 bytes each, as many as the products themselves take at their full rate; and by the power limit: of
-// operands that are all zeros the first takes 496 us, the second 1818, and 4 products of 8192 x 4096 x 8192 428 us instead of 546.
+// 590 - 600 us over the same buffers once the power limit has settled (710 in the first 20 passes), without loads 531, without stores
+// 472, without both 406 (of which the products alone would be 281 at the 6.6 PFLOP/s that the power limit leaves them on random
+// operands).  On 16 x 8192 x 2048 x 16384: 2140 - 2220 us (4000 TFLOP/s); 4 products of 8192^3: 960 us (4580).  Beside the stores it
+// is bound by the LDS and by how its reads and the products follow each other: per 128 of K its wavefronts read 96 KB from it and
+// 32 KB are put in, 1024 of its cycles at 128 bytes each, as many as the products themselves take at their full rate, and two
+// wavefronts per SIMD with two barriers a stage do not hide all of one behind the other.  On operands that are all zeros, where
+// power is no limit, the second takes 1818 us, of which products alone would take 1011 at the 8.7 PFLOP/s that a loop of them reaches
+// on constants: some 800 us are the schedule's, 300 - 400 the power limit's.  (The first on zeros: 496 us; 4 products of
+// 8192 x 4096 x 8192: 428 us instead of 546.)
 // What did not help: groups of 4, 16 or 32 feature tiles in the order of the tiles (3 - 5 us slower); wavefronts' priorities
 // (nothing); four wavefronts of 128 x 128 with the accumulators in the AGPRs (642 -> 701 us; nobody fills the waits).
 constexpr int TW = 8;                         // wavefronts
@@ -683,7 +695,8 @@ __global__ __launch_bounds__(TW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   // Block b runs on XCD b % 8 and takes every (gridDim / 8)-th of that XCD's share of the tiles, a run of them in an order
   // that goes through 8 feature tiles for each token tile: the W tiles stay in the XCD's L2 while the tokens pass.
   // The last feature tile is moved back inside the matrix; what it shares with its neighbour is the same in both.
-  // K is walked from a stage of the tile's own, so that the CUs that share x or W ask for different lines at any one time.
+  // K is walked from a stage of the tile's own, so that the CUs that share x or W ask for different lines at any one time.  The order of
+  // a result's sum so depends on its tile: the last bit of a token's float32 results on where in the batch the token lies.
   struct At { int layer, tm, m0, n0, tn, rot; };
   auto locate = [&](int t) {
     At at;
@@ -987,8 +1000,8 @@ template <typename T, int GROUPS> __device__ __forceinline__ void mx_tile_side(c
 template <typename T, int GROUPS> __global__ __launch_bounds__(256) void k_mx_tile_side(MxSide a) {
   mx_tile_side<T, GROUPS>(a, blockIdx.x, gridDim.x / a.stages, blockIdx.y);
 }
-// The same for the weights beside the quantisation of x, neither of which waits for the other: 8.2 us for 77 tokens of 12 x 24576 x 768,
-// 150 us for 8192 of 16 x 16384 x 2048 (0.72 GB); as two launches, a thread going through a tile's stages, 5.0 + 7.6 and 136 + 38 us.
+// The same for the weights beside the quantisation of x, neither of which waits for the other: 7 us for 77 tokens of 12 x 24576 x 768,
+// 148 us for 8192 of 16 x 16384 x 2048 (0.72 GB); as two launches, a thread going through a tile's stages, 5.0 + 7.6 and 136 + 38 us.
 template <typename T, bool VEC> __global__ __launch_bounds__(256) void k_mx_tile_inputs(MxSide a, int tiles, MxWrite x) {
   const int side = tiles * a.stages;
   if ((int)blockIdx.x < side) mx_tile_side<T, 8>(a, blockIdx.x, tiles, blockIdx.y);
@@ -1092,8 +1105,13 @@ int mx_read(int dtype, int fmt, const void *codes, const uint8_t *scales, const 
 // How a shape is computed.  Up to 64 tokens, as long as their rows leave room in LDS for two workgroups per CU, by the kernel for few:
 // W is read once then.  Beyond by tiles, where there are whole feature tiles and rows of the result lie at whole words (buffer
 // stores); else by the kernel for few in groups of tokens.  12 layers, d 768, F 24576, bf16, kernel for few against tiles, us, x
-// quantised in the call: 26 against 47 at 1 token, 30 / 45 at 17, 34 / 46 at 33, 40 / 46 at 64, 63 / 50 at 77, 75 / 50 at 128, 148 / 57
-// at 256; 16 layers, d 2048, F 16384: 78 / 97 at 17, 95 / 99 at 64.
+// quantised in the call: 26 against 49 at 1 token, 31 / 48 at 17, 35 / 47 at 33, 41 / 47 at 64, 63 / 49 at 77, 75 / 50 at 128, 148 / 59
+// at 256; 16 layers, d 2048, F 16384: 75 / 103 at 1, 81 / 103 at 17, 98 / 105 at 64.
+// Results of 16 bits with an odd F have no whole words in their rows, and go
+// through the weights once per 128 tokens: 12 layers, d 768, bf16, F 24575
+// against 24576: 192 / 56 us at 256 tokens, 699 / 171 at 1024, 2127 / 627 at 4096.  Rows that LDS does not hold for even 16 tokens
+// (d above about 9600) go by tiles from one token on: 4 layers, F 4096, one token: 41 us at d 9216 (1.97 TB/s of weights), 63 at 9728,
+// 77 at 12288 (1.40), where 32 tokens take 78.
 bool mx_tiles_fit(int64_t F, const void *pre, int64_t ps, int64_t pre_row, int64_t e) {
   return ((uintptr_t)pre & 3u) == 0 && ps * e % 4 == 0 && pre_row * e % 4 == 0 && F * e % 4 == 0 && pre_row * e <= (1 << 22);
 }

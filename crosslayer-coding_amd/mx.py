@@ -205,7 +205,9 @@ def refresh(x: torch.Tensor, out: MXTensor, state: torch.Tensor, changed: torch.
 def project(x: Union[torch.Tensor, MXTensor], w: MXTensor, b: Optional[torch.Tensor] = None,
             out: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None, ws=None) -> torch.Tensor:
     """``pre[l] = x[l] @ w[l].T + b[l]`` on the 4-bit matrix cores: ``w`` [L, F, d] in mxfp4, ``x`` [L, T, d] quantised to
-    mxfp4 on the way in (or an `MXTensor` that is), fp32 sums, one rounding.  ``b`` [L, F]; [T, d] with w [F, d] and b [F]
+    mxfp4 on the way in (or an `MXTensor` that is), fp32 sums, one rounding.  The order of the sums goes by the shapes, where
+    ``out`` begins and where in the batch a row lies: calls repeat bit by bit, the same token at another place may differ in its last
+    float32 bit.  ``b`` [L, F]; [T, d] with w [F, d] and b [F]
     is one layer.  The result has x's type, or ``out``'s / b's / ``dtype`` where x comes quantised.  ``ws``: an
     `engine.Workspace` to take the scratch memory from."""
     if w.fmt != "mxfp4" or len(w.shape) not in (2, 3):

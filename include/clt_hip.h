@@ -914,7 +914,9 @@ int clt_feed_gather(const void *src, int src_dtype, int64_t src_rows, int64_t sr
  * clt_mx_encode: pre[l] = x[l] . w[l]^T + b[l] with both operands in CLT_MXFP4: exact products, fp32 sums, the bias
  *   added in fp32, one rounding to dtype (that of bias and pre; bias may be NULL).  w [L][F] rows of d elements.  x is
  *   [L][T][d] values of dtype, layers x_layer_stride apart, which the call quantises, when x_scales is NULL; else its
- *   codes and scales [L][T].  pre rows are pre_row_stride >= F elements apart, layers pre_layer_stride.
+ *   codes and scales [L][T].  The order of the sums depends on the shapes, the result's alignment
+ *   and pitch, and a row's place in the batch, on nothing else.
+ *   pre rows are pre_row_stride >= F elements apart, layers pre_layer_stride.
  *   What clt_encode computes from 16- or 32-bit operands (clt/models/parallel.py:286).  workspace: 16-byte aligned,
  *   clt_mx_encode_workspace_bytes (may be 0 when x comes quantised).  T up to 16 * 65535, F up to 2^30, L up to 32767,
  *   (T + F / 4) * ceil(d / 32) below 2^30 (CLT_ERR_RANGE).
