@@ -28,8 +28,9 @@ def _true(model, inputs, x):
     b = torch.stack([e.bias_param.detach() for e in model.encoder_module.encoders]).cpu().double().unsqueeze(1)
     xq, wq = orc.round_trip(x.cpu(), "mxfp4"), orc.round_trip(w, "mxfp4")
     want = xq @ wq.transpose(1, 2) + b
-    tol = (xq.abs() @ wq.abs().transpose(1, 2) + b.abs()) * (w.shape[-1] + 1) * 2.0 ** -23 + want.abs() * torch.finfo(model.dtype).eps / 2 * 1.01 + 1e-30
     pre, _ = model._encode_all_layers(inputs)
+    # half a step of the type that the results have: a model that was just moved to another type knows its own with the next call
+    tol = (xq.abs() @ wq.abs().transpose(1, 2) + b.abs()) * (w.shape[-1] + 1) * 2.0 ** -23 + want.abs() * torch.finfo(pre[0].dtype).eps / 2 * 1.01 + 1e-30
     for l in inputs:
         assert bool(((pre[l].cpu().double() - want[l]).abs() <= tol[l]).all()), l
 
@@ -229,3 +230,107 @@ def test_quantise_again_shows_a_write_that_the_samples_miss(dev):
         _true(model, inputs, x)
         model.encoder_module.encoders[2].weight[5, 77] = -50.0       # not past the version counter: shows by itself
         _true(model, inputs, x)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("L,T,F,d,row,gap,at", [
+    (2, 300, 520, 320, 528, 64, 0), (2, 300, 512, 640, 576, 0, 64), (1, 77, 257, 768, 260, 0, 2), (2, 5, 100, 96, 101, 7, 1),
+    (2, 513, 301, 160, 301, 3, 1), (3, 600, 768, 256, 1024, 256, 0), (1, 64, 1000, 2048, 1001, 0, 0)])
+def test_project_into_rows_of_a_larger_buffer(dev, dtype, L, T, F, d, row, gap, at):
+    """The C entry: rows ``row`` elements apart, layers ``gap`` more, the first at an address of its own; what lies between stays."""
+    lib = cca._native.load()
+    x = _whole_numbers((L, T, d), 0, T).to(dtype).to(dev)
+    w = cca.mx.quantise(_whole_numbers((L, F, d), 1, F).to(dev))
+    b = (torch.arange(L * F).reshape(L, F) % 200 - 100).to(dtype).to(dev)
+    layer = T * row + gap
+    buf = torch.full((at + L * layer + 500,), 7.0, dtype=dtype, device=dev)
+    nbytes = lib.clt_mx_encode_workspace_bytes(T, d, F, L, 0)
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+    code = lib.clt_mx_encode(x.data_ptr(), None, w.codes.data_ptr(), w.scales.data_ptr(), b.data_ptr(), buf.data_ptr() + at * buf.element_size(),
+                             T, d, F, L, T * d, F, layer, row, cca._native.dtype_code(dtype), ws.data_ptr(), nbytes, cca._native.current_stream(dev))
+    assert code == 0
+    want = torch.full_like(buf, 7.0)
+    w64 = w.dequantise().double()
+    for l in range(L):
+        pre = (torch.mm(x[l].double(), w64[l].t().contiguous()) + b[l].double()).to(dtype)
+        want[at + l * layer:at + l * layer + T * row].view(T, row)[:, :F] = pre
+    assert torch.equal(buf, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8", "mxint8"])
+@pytest.mark.parametrize("n,d,row,at", [(9, 96, 96, 1), (300, 64, 72, 0), (5, 100, 103, 3), (2000, 768, 1024, 0), (1500, 768, 776, 8), (1, 33, 0, 5)])
+def test_rows_apart_and_at_any_address_come_and_go(dev, dtype, fmt, n, d, row, at):
+    """The C entries: quantised from rows of a larger buffer, given out into rows of another, which keeps what lies between."""
+    lib = cca._native.load()
+    code, stream = cca._native.dtype_code(dtype), cca._native.current_stream(dev)
+    g = torch.Generator().manual_seed(n + d)
+    src = torch.randn(at + n * max(row, d) + 64, generator=g).to(dtype).to(dev)
+    pitch, blocks = cca.mx.row_layout(d, fmt)
+    codes = torch.full((n + 1, pitch), 9, dtype=torch.uint8, device=dev)
+    scales = torch.full((n + 1, blocks), 9, dtype=torch.uint8, device=dev)
+    f = cca.mx.FORMATS[fmt]
+    assert lib.clt_mx_quantise(src.data_ptr() + at * src.element_size(), n, d, row, code, f, codes.data_ptr(), scales.data_ptr(), stream) == 0
+    rows = src[at:].as_strided((n, d), (max(row, d) if n > 1 else d, 1), at).cpu()
+    c, s = orc.quantise(rows, fmt)
+    assert torch.equal(codes[:n].cpu(), c) and torch.equal(scales[:n].cpu(), s)
+    assert bool((codes[n] == 9).all()) and bool((scales[n] == 9).all())
+    out = torch.full_like(src, 7.0)
+    assert lib.clt_mx_dequantise(codes.data_ptr(), scales.data_ptr(), n, d, f, out.data_ptr() + at * out.element_size(), row, code, stream) == 0
+    want = torch.full_like(src, 7.0)
+    want.as_strided((n, d), (max(row, d) if n > 1 else d, 1), at).copy_(orc.dequantise(c, s, fmt, d).to(dtype))
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("fn", ["batchtopk", "topk", "jumprelu", "relu"])
+def test_captured_forwards_of_every_activation(dev, fn, dtype):
+    model, inputs, x = _model(dev, T=70, dtype=dtype, fn=fn)
+    model.quantise_encoder()
+    with torch.no_grad():
+        g, out = _capture(model, inputs)
+        for trial in range(3):
+            x.copy_(torch.roll(x, 1, dims=1) * 1.25)
+            if trial == 1:
+                model.encoder_module.encoders[2].weight.data.mul_(0.5)
+            if trial == 2:
+                model.encoder_module.encoders[0].weight.mul_(-1.0)
+            g.replay()
+            torch.cuda.synchronize()
+            got = {l: v.clone() for l, v in out.items()}
+            pre, _ = model._encode_all_layers(inputs)
+            want = model(inputs)
+            for l in got:
+                # eager threshold models may decode by another route, which adds in another order
+                scale = float(want[l].float().abs().max())
+                assert float((got[l].float() - want[l].float()).abs().max()) <= (2.0 ** -6 if fn in ("jumprelu", "relu") else 0.0) * scale, (trial, l)
+        _true(model, inputs, x)
+
+
+def test_a_copied_model_has_a_copy_of_its_own(dev):
+    import copy
+
+    model, inputs, x = _model(dev)
+    model.quantise_encoder()
+    with torch.no_grad():
+        want = {l: v.clone() for l, v in model(inputs).items()}
+        twin = copy.deepcopy(model)
+        twin.encoder_module.encoders[1].weight.data.neg_()
+        _true(twin, inputs, x)
+        _true(model, inputs, x)
+        twin.dequantise_encoder()
+        again = model(inputs)
+        assert all(torch.equal(again[l], want[l]) for l in want)
+
+
+def test_a_model_of_another_type_or_device_and_back(dev):
+    model, inputs, x = _model(dev, dtype="float32")
+    model.quantise_encoder()
+    with torch.no_grad():
+        model(inputs)
+        model.to(torch.bfloat16)
+        _true(model, {l: v.bfloat16() for l, v in inputs.items()}, x.bfloat16())
+        model.cpu()
+        model.encoder_module.encoders[0].weight.data.neg_()
+        model.to(dev)
+        _true(model, {l: v.bfloat16() for l, v in inputs.items()}, x.bfloat16())
